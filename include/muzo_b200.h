@@ -340,6 +340,38 @@ int muzo_attention_max(const void* q, const void* k, const void* v, void* out, i
                        const int32_t* d_key_lo, const int32_t* d_key_hi, float* smax, int32_t* d_valid,
                        int32_t* d_status, void* stream);
 
+/* muzo_attention_max that also keeps, when lse is non-NULL, the natural logarithm of each row's sum
+ * of exp(scale * logit) over its visible keys, lse[b][h][i] (float[B * Hq * Sq], -inf for a row
+ * that sees none): the statistic muzo_attention_backward recomputes the probabilities from. The
+ * scale must then be positive. D may be any multiple of 8 up to 128 (here and in
+ * muzo_attention_max); Sk = 0 is allowed (K and V may then be NULL) and writes zeros. */
+int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* out, float* lse, int dtype,
+                           int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+                           int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                           int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                           int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+                           int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s, int causal, float scale,
+                           const int32_t* d_key_lo, const int32_t* d_key_hi, float* smax, int32_t* d_valid,
+                           int32_t* d_status, void* stream);
+
+/* Gradients of that attention (no counterpart in the reference, which trains without gradients):
+ * with P = exp(scale * Q K^T - lse) over the visible pairs, dP = dO V^T, delta = rowsum(dO * O) and
+ * dS = P * (dP - delta):  dV = P^T dO, dK = scale * dS^T Q, dQ = scale * dS K, dK and dV summed over
+ * the Hq / Hkv query heads of a key head. P and dS enter the products in the input type, sums are
+ * fp32. Nothing is added atomically: equal calls give equal bits. Any of dq, dk, dv may be NULL
+ * (dq alone, or dk and dv, skip the other's work). `strides` (host memory, 24 entries): the element
+ * strides (batch, head, sequence) of q, k, v, out, dout, dq, dk, dv, all multiples of 8 and, for the
+ * inputs, nonzero; D contiguous, bases 16-byte aligned. d_workspace: device memory of at least
+ * muzo_attention_backward_workspace(...) bytes (negative: a shape this call refuses), 16-byte
+ * aligned, that no other call uses until this one has finished. d_status as in muzo_attention_max. */
+int64_t muzo_attention_backward_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q,
+                                          int64_t seq_k, int64_t head_dim);
+int muzo_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                            const float* lse, void* dq, void* dk, void* dv, int dtype, int64_t batch, int64_t hq,
+                            int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim, const int64_t* strides,
+                            int causal, float scale, const int32_t* d_key_lo, const int32_t* d_key_hi,
+                            void* d_workspace, int64_t workspace_bytes, int32_t* d_status, void* stream);
+
 /* Row-group scaling of a projection weight (qk_clip.py:287-308): rows
  * [g*rows_per_group, (g+1)*rows_per_group) are multiplied by factors[g] (already rounded to
  * the weight dtype) when mask[g] != 0. w is row-major [groups*rows_per_group, cols]. */

@@ -24,23 +24,21 @@
 // Every wait is bounded; on timeout the kernel records a code in the status word, raises its
 // abort flag, drains its loads and MMAs, frees TMEM and returns.
 #include <atomic>
+#include <cfloat>
 #include <cstdlib>
 
-#include "tcgen05_common.cuh"
+#include "attention_common.cuh"
 
 namespace muzo {
 namespace {
 
 using namespace tc;
+using namespace attn;
 
-constexpr int AM = 128;          // query rows per query tile (UMMA M)
 constexpr int AMB = 2 * AM;      // query rows per CTA: two query tiles share each K / V tile
-constexpr int AN = 128;          // keys per tile: UMMA N of S, the K of P V
-constexpr int ABK = 64;          // 128-byte swizzle row of 16-bit elements
 constexpr int A_THREADS = 352;   // warp 0 TMA of Q and K, warp 1 MMA, warps 2..9 softmax (two streams
                                  // of four warps, one warp per TMEM lane quarter), warp 10 TMA of V
 constexpr int K_STAGES = 1;      // K ring depth (tile j uses K stage j % K_STAGES)
-constexpr int SUB_BYTES = 128 * ABK * 2;     // one swizzled block of 128 rows x 64 elements (16 KB)
 constexpr int BOX_BYTES = 64 * ABK * 2;      // one 64 x 64 box of the MN-major V operand (8 KB)
 constexpr uint32_t TMEM_COLS = 512;          // S of each stream at 0 and 128, O of each stream from 256
 constexpr float kRescaleLog2 = 8.0f;          // lazy rescale threshold: P stays below 2^8
@@ -70,6 +68,8 @@ struct AttnArgs {
   const int32_t* key_hi;       // per batch, or null (Sk)
   void* out;
   int64_t o_sb, o_sh, o_ss;    // output strides in elements; D contiguous
+  int hd;                      // head dimension (at most D: the tiles' further columns hold zeros)
+  float* lse;                  // log of each row's sum of exp(scaled logit), [B][Hq][Sq], or null
   int* enc;                    // per-head running maximum of the raw logits (order-preserving ints), or null
   int32_t* valid;
   int32_t* status;
@@ -78,12 +78,6 @@ struct AttnArgs {
 __device__ __forceinline__ int encode_max(float f) {
   const int b = __float_as_int(f);
   return b >= 0 ? b : b ^ 0x7fffffff;
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Work item -> (batch, head, block of 256 queries); the longest query blocks (last, when causal) first.
@@ -99,10 +93,7 @@ __device__ __forceinline__ void attn_item(const AttnArgs& g, int64_t t, int& b, 
 // no row inside the sequence or no visible key).
 __device__ __forceinline__ void attn_tiles(const AttnArgs& g, int b, int qb, int64_t& lo, int64_t& hi, int& t0,
                                            int& n0, int& n1) {
-  lo = g.key_lo ? g.key_lo[b] : 0;
-  hi = g.key_hi ? g.key_hi[b] : g.sk;
-  if (lo < 0) lo = 0;
-  if (hi > g.sk) hi = g.sk;
+  key_range(g.key_lo, g.key_hi, g.sk, b, lo, hi);
   t0 = static_cast<int>(lo / AN);
   int n[2];
   for (int t = 0; t < 2; ++t) {
@@ -388,7 +379,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const float mt2 = mt * g.scale_log2;
       float alpha = 1.0f;
       bool rescale = false;
-      if (mt2 > m_run + kRescaleLog2) {
+      if (mt2 > m_run + kRescaleLog2 || mt != mt) {   // a NaN logit makes its row NaN
         alpha = m_run == -INFINITY ? 0.0f : fast_exp2(m_run - mt2);
         rescale = u > 0;
         m_run = mt2;
@@ -457,6 +448,22 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
       }
       l_run = l_run * alpha + (((lsum[0] + lsum[1]) + (lsum[2] + lsum[3])) + ((lsum[4] + lsum[5]) + (lsum[6] + lsum[7])));
+      // keys outside [lo, hi) that share a tile with visible ones: their P is 0, but 0 times a
+      // non-finite V would still reach O, so their V rows are cleared before P V reads them
+      if (lo > key0 || hi < (g.sk < key0 + AN ? g.sk : key0 + AN)) {
+        const int stage = u % VS;
+        if (!mbar_wait(v_full + stage, static_cast<uint32_t>((u / VS) & 1))) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (key0 + r < lo || key0 + r >= hi) {
+          uint8_t* vrow = sV + stage * L::V_BYTES + (r >> 6) * (NKB * BOX_BYTES) + (r & 63) * 128;
+#pragma unroll
+          for (int dc = 0; dc < NKB; ++dc)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(vrow + dc * BOX_BYTES + 16 * e) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       __syncwarp();
@@ -473,6 +480,9 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (ok) {
       // O / l of this row (zeros for a row without a visible key or a tile without one)
       const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+      if (g.lse != nullptr && row_in)
+        g.lse[(static_cast<int64_t>(b) * g.hq + h) * g.sq + row] =
+            l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * 0.6931471805599453f;
       uint16_t* orow = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(b) * g.o_sb +
                        static_cast<int64_t>(h) * g.o_sh + row * g.o_ss;
 #pragma unroll 1
@@ -487,6 +497,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (row_in) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
+            if (c * 32 + 8 * q >= g.hd) break;
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -532,23 +543,6 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   }
 }
 
-// 4-D tensor map over [B][H][S][D] (element strides ss, sh, sb; D contiguous), box 64 x rows.
-int encode_attn_map(CUtensorMap* map, const void* base, int dtype, int64_t d, int64_t s, int64_t h, int64_t b,
-                    int64_t ss, int64_t sh, int64_t sb, int rows) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return MUZO_ERR_UNSUPPORTED;
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(s), static_cast<cuuint64_t>(h),
-                        static_cast<cuuint64_t>(b)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss * 2), static_cast<cuuint64_t>(sh * 2),
-                           static_cast<cuuint64_t>(sb * 2)};
-  cuuint32_t box[4] = {ABK, static_cast<cuuint32_t>(rows), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType dt = dtype == MUZO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult res = fn(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return res == CUDA_SUCCESS ? MUZO_OK : MUZO_ERR_ARG;
-}
-
 template <int FMT, int D>
 int launch_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& g,
                 cudaStream_t s) {
@@ -582,8 +576,6 @@ __global__ void finalize_attn_max_kernel(int* enc, int n, int dtype, float scale
   reinterpret_cast<float*>(enc)[i] = v;
 }
 
-bool aligned16p(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace muzo
 
@@ -591,19 +583,20 @@ using namespace muzo;
 
 extern "C" {
 
-int muzo_attention_max(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
-                       int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* out, float* lse, int dtype, int64_t batch,
+                           int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                        int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
                        int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
                        int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
                        int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s, int causal, float scale,
                        const int32_t* d_key_lo, const int32_t* d_key_hi, float* smax, int32_t* d_valid,
                        int32_t* d_status, void* stream) {
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || d_status == nullptr || batch < 0 ||
-      hq <= 0 || hkv <= 0 || hq % hkv != 0 || seq_q < 0 || seq_k < 0 || (smax != nullptr && d_valid == nullptr))
+  if (q == nullptr || ((k == nullptr || v == nullptr) && seq_k != 0) || out == nullptr || d_status == nullptr || batch < 0 ||
+      hq <= 0 || hkv <= 0 || hq % hkv != 0 || seq_q < 0 || seq_k < 0 ||
+      (smax != nullptr && d_valid == nullptr) || (lse != nullptr && !(scale > 0.0f && scale <= FLT_MAX)))
     return MUZO_ERR_ARG;
   if (dtype != MUZO_BF16 && dtype != MUZO_F16) return MUZO_ERR_DTYPE;
-  if (head_dim != 64 && head_dim != 128) return MUZO_ERR_UNSUPPORTED;
+  if (head_dim < 8 || head_dim % 8 != 0 || head_dim > 128) return MUZO_ERR_UNSUPPORTED;
   const int64_t strides[12] = {q_stride_b, q_stride_h, q_stride_s, k_stride_b, k_stride_h, k_stride_s,
                                v_stride_b, v_stride_h, v_stride_s, o_stride_b, o_stride_h, o_stride_s};
   for (int64_t st : strides)
@@ -620,11 +613,16 @@ int muzo_attention_max(const void* q, const void* k, const void* v, void* out, i
   if (items > 0) {
     if (items > 0x7fffffffLL) return MUZO_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv;
+    if (seq_k == 0) {   // no key tile is loaded: any valid map will do
+      k = v = q;
+      k_stride_b = v_stride_b = k_stride_h = v_stride_h = k_stride_s = v_stride_s = 8;
+    }
+    const int64_t map_keys = seq_k > 0 ? seq_k : 1;
     int st = encode_attn_map(&mq, q, dtype, head_dim, seq_q, hq, batch, q_stride_s, q_stride_h, q_stride_b, AM);
     if (st != MUZO_OK) return st;
-    st = encode_attn_map(&mk, k, dtype, head_dim, seq_k, hkv, batch, k_stride_s, k_stride_h, k_stride_b, AN);
+    st = encode_attn_map(&mk, k, dtype, head_dim, map_keys, hkv, batch, k_stride_s, k_stride_h, k_stride_b, AN);
     if (st != MUZO_OK) return st;
-    st = encode_attn_map(&mv, v, dtype, head_dim, seq_k, hkv, batch, v_stride_s, v_stride_h, v_stride_b, 64);
+    st = encode_attn_map(&mv, v, dtype, head_dim, map_keys, hkv, batch, v_stride_s, v_stride_h, v_stride_b, 64);
     if (st != MUZO_OK) return st;
     AttnArgs g;
     g.sq = seq_q; g.sk = seq_k; g.shift = seq_k - seq_q;
@@ -634,17 +632,32 @@ int muzo_attention_max(const void* q, const void* k, const void* v, void* out, i
     g.scale_log2 = scale * 1.4426950408889634f;
     g.key_lo = d_key_lo; g.key_hi = d_key_hi;
     g.out = out; g.o_sb = o_stride_b; g.o_sh = o_stride_h; g.o_ss = o_stride_s;
+    g.hd = static_cast<int>(head_dim); g.lse = lse;
     g.enc = enc; g.valid = d_valid; g.status = d_status;
     if (dtype == MUZO_BF16)
-      st = head_dim == 64 ? launch_attn<1, 64>(mq, mk, mv, g, s) : launch_attn<1, 128>(mq, mk, mv, g, s);
+      st = head_dim <= 64 ? launch_attn<1, 64>(mq, mk, mv, g, s) : launch_attn<1, 128>(mq, mk, mv, g, s);
     else
-      st = head_dim == 64 ? launch_attn<0, 64>(mq, mk, mv, g, s) : launch_attn<0, 128>(mq, mk, mv, g, s);
+      st = head_dim <= 64 ? launch_attn<0, 64>(mq, mk, mv, g, s) : launch_attn<0, 128>(mq, mk, mv, g, s);
     if (st != MUZO_OK) return st;
   }
   if (enc != nullptr)
     finalize_attn_max_kernel<<<static_cast<unsigned>((hq + 255) / 256), 256, 0, s>>>(enc, static_cast<int>(hq), dtype,
                                                                                      scale);
   return launch_status();
+}
+
+int muzo_attention_max(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
+                       int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+                       int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                       int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                       int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+                       int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s, int causal, float scale,
+                       const int32_t* d_key_lo, const int32_t* d_key_hi, float* smax, int32_t* d_valid,
+                       int32_t* d_status, void* stream) {
+  return muzo_attention_max_lse(q, k, v, out, nullptr, dtype, batch, hq, hkv, seq_q, seq_k, head_dim, q_stride_b,
+                                q_stride_h, q_stride_s, k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h,
+                                v_stride_s, o_stride_b, o_stride_h, o_stride_s, causal, scale, d_key_lo, d_key_hi, smax,
+                                d_valid, d_status, stream);
 }
 
 }  // extern "C"

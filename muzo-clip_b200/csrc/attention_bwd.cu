@@ -1,0 +1,821 @@
+// Attention's backward pass on the tensor cores, recomputing the probabilities from the row
+// statistics that the forward kept (attention.cu, the lse output):
+//   P_ij = exp(c q_i . k_j - lse_i)      delta_i = dO_i . O_i       dP_ij = dO_i . v_j
+//   dS_ij = P_ij (dP_ij - delta_i)
+//   dV_j = sum_i P_ij dO_i     dK_j = c sum_i dS_ij q_i     dQ_i = c sum_j dS_ij k_j
+// over the visible pairs (key_lo[b] <= j < key_hi[b] and, when causal, j <= i + Sk - Sq), dK and dV
+// summed over the query heads of a key head.
+//
+// One launch of two kinds of CTA (ten warps), neither of which adds to memory atomically, so that
+// equal calls give equal bits:
+//   key CTAs    own 128 keys of one key head and walk the query tiles of its heads:
+//               S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q;
+//   query CTAs  own 128 queries of one head and walk the key tiles:
+//               S = Q K^T, dP = dO V^T, dQ += dS K.
+// Forming S and dP twice costs 7 products instead of 5, and saves the fp32 dQ that would have to be
+// added up in memory in a fixed order.
+#include <atomic>
+#include <cfloat>
+
+#include "attention_common.cuh"
+
+namespace muzo {
+namespace {
+
+using namespace tc;
+using namespace attn;
+
+constexpr int B_THREADS = 320;   // warp 0 TMA, warp 1 MMA, warps 2..9 probabilities: two warps per TMEM
+                                 // lane quarter, 64 of the tile's 128 columns each
+constexpr uint32_t B_TMEM_COLS = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct BwdLayout {
+  static constexpr int NKB = D / ABK;
+  static constexpr int TILE_BYTES = NKB * SUB_BYTES;   // 128 rows of one operand
+  static constexpr int TILES = 7;                      // key CTA: K, V, 2 Q, 2 dO, statistics; query CTA: Q, dO, 3 K, 2 V
+  static constexpr int BAR_BYTES = 256;
+  static constexpr int NEED = TILES * TILE_BYTES + BAR_BYTES + 1024;
+  static constexpr int SMEM_BYTES = NEED > 116 * 1024 ? NEED : 116 * 1024;   // one CTA per SM: it takes all of TMEM
+};
+
+struct BwdArgs {
+  int64_t sq, sk, shift;
+  int batch, hq, hkv, group, nqt, nkt, causal, hd, parts;
+  int64_t key_items, query_items;
+  float scale, scale_log2;
+  const int32_t* key_lo;
+  const int32_t* key_hi;
+  const float* stats;    // [B * Hq][nqt][2][128]: -lse in log2 units (-inf: no key seen, or no such row), delta
+  float* partial;        // [parts][B * Hkv][nkt * 128][2][D] sums of dV and c dK, or null when parts == 1
+  uint16_t *dq, *dk, *dv;   // any may be null
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int32_t* status;
+};
+
+// D = A B with A from TMEM (128 lanes, 8 columns of packed 16-bit pairs per K = 16) and B from shared memory.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// `bytes` (a multiple of 16) of contiguous global memory into shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return FMT == 1 ? pack_bf16(lo, hi) : pack_half(lo, hi);
+}
+
+// One lane waits for the barrier, the warp shares the answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int lane, const int* abort_flag) {
+  bool ready = true;
+  if (lane == 0) ready = mbar_wait(bar, parity) && !*reinterpret_cast<const volatile int*>(abort_flag);
+  return __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
+}
+
+// Query tiles [first, first + count) that see a key of key tile kt in batch row b.
+__device__ __forceinline__ void key_tile_queries(const BwdArgs& g, int b, int kt, int64_t& lo, int64_t& hi, int& first,
+                                                 int& count) {
+  key_range(g.key_lo, g.key_hi, g.sk, b, lo, hi);
+  first = 0;
+  count = 0;
+  const int64_t key0 = static_cast<int64_t>(kt) * AN;
+  const int64_t a = key0 > lo ? key0 : lo;                        // first and last visible key of the tile
+  const int64_t z = key0 + AN < hi ? key0 + AN : hi;
+  if (a >= z) return;
+  if (g.causal) {
+    const int64_t q = a - g.shift;                                // the first query that sees key a
+    if (q >= g.sq) return;
+    first = q > 0 ? static_cast<int>(q / AM) : 0;
+  }
+  count = g.nqt - first;
+}
+
+// Key tiles [first, first + count) that query tile qt of batch row b sees.
+__device__ __forceinline__ void query_tile_keys(const BwdArgs& g, int b, int qt, int64_t& lo, int64_t& hi, int& first,
+                                                int& count) {
+  key_range(g.key_lo, g.key_hi, g.sk, b, lo, hi);
+  int64_t end = hi;
+  if (g.causal) {
+    const int64_t q = static_cast<int64_t>(qt) * AM + AM - 1;
+    const int64_t last = (q < g.sq - 1 ? q : g.sq - 1) + g.shift + 1;
+    if (last < end) end = last;
+  }
+  first = static_cast<int>(lo / AN);
+  count = end > lo ? static_cast<int>((end + AN - 1) / AN) - first : 0;
+}
+
+// 32 accumulator columns of this thread's row, times f, as 16-bit values at `dst` (columns col0.. of hd).
+template <int FMT>
+__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[32], float f, int col0, int hd) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (col0 + 8 * q >= hd) break;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = pack16<FMT>(__uint_as_float(v[8 * q + 2 * e]) * f, __uint_as_float(v[8 * q + 2 * e + 1]) * f);
+    *reinterpret_cast<uint4*>(dst + col0 + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Barriers of both kinds of CTA.
+enum : int {
+  kFull = 0,        // key CTA: K, V, Q[2], dO[2]; query CTA: Q, dO, K[3], V[2]
+  kEmpty = 7,       // key CTA: Q[2], dO[2] (at 2 and 4); query CTA: K[3], V[2] (at 2 and 5)
+  kS = 14,          // S computed (query CTA: two, by buffer)
+  kDp = 16,         // dP computed
+  kP = 17,          // key CTA: P written and S read
+  kDs = 18,         // dS written and dP read
+  kDone = 19,
+  kDrain = 20,
+  kStall = 21,
+  kBars = 22
+};
+
+// Loads issued by the producer thread: which full barriers are armed, and with which parity.
+struct Armed {
+  uint32_t mask = 0, parity = 0;
+  __device__ __forceinline__ void arm(uint64_t* bars, int i, uint32_t phase, uint32_t bytes) {
+    mbar_arrive_expect_tx(bars + kFull + i, bytes);
+    mask |= 1u << i;
+    parity = (parity & ~(1u << i)) | (phase << i);
+  }
+  __device__ __forceinline__ void wait_all(uint64_t* bars) const {
+    for (int i = 0; i < 7; ++i)
+      if (mask & (1u << i)) mbar_wait(bars + kFull + i, (parity >> i) & 1u);
+  }
+};
+
+template <int NKB>
+__device__ __forceinline__ void load_tile(const CUtensorMap* map, uint64_t* bar, uint8_t* dst, int row, int h, int b) {
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb) tma_load_4d(map, bar, dst + kb * SUB_BYTES, kb * ABK, row, h, b);
+}
+
+// D (128 x 128) = A B^T, both operands K-major tiles of D columns in shared memory.
+template <int NKB>
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, const uint8_t* a, const uint8_t* b, uint32_t idesc) {
+  const uint32_t sa = smem_u32(a), sb = smem_u32(b);
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+    for (int k = 0; k < ABK / 16; ++k)
+      umma_f16(tmem_d, make_sdesc(sa + kb * SUB_BYTES + k * 32, 16, 1024), make_sdesc(sb + kb * SUB_BYTES + k * 32, 16, 1024),
+               idesc, (kb > 0 || k > 0) ? 1u : 0u);
+}
+
+// D (128 x NKB*64) (+)= A B: A packed in TMEM (columns 0..31 for K rows 0..63, 64..95 for 64..127),
+// B a tile of 128 rows in shared memory read MN-major.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const uint8_t* b, uint32_t idesc, bool accumulate) {
+  const uint32_t sb = smem_u32(b);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    umma_f16_ts(tmem_d, tmem_a + (k < 4 ? 8 * k : 32 + 8 * k), make_sdesc(sb + k * (16 * 128), SUB_BYTES, 1024), idesc,
+                (accumulate || k > 0) ? 1u : 0u);
+}
+
+// What a role that gave up does: the first code stays in the status word.
+__device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int code) {
+  atomicCAS(g.status, kErrNone, code);
+  atomicExch(abort_flag, 1);
+}
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(B_THREADS, 1)
+attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, BwdArgs g) {
+  using L = BwdLayout<D>;
+  constexpr int NKB = L::NKB;
+  constexpr int TILE = L::TILE_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::TILES * TILE);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kBars);
+  int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stall = *reinterpret_cast<volatile int*>(g.status + 1);
+  const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBars; ++i) mbar_init(bars + i, (i == kP || i == kDs) ? 8 : 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(B_TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  constexpr uint32_t idesc_s = make_idesc_fmt(128, 128, false, false, FMT);   // S, dP: both operands K-major
+  constexpr uint32_t idesc_g = make_idesc_fmt(128, D, false, true, FMT);      // gradients: B MN-major
+  const int quarter = warp & 3, half = (warp - 2) >> 2;
+  const int r = 32 * quarter + lane;                                          // row of the tile == TMEM lane
+  const uint32_t lane_addr = static_cast<uint32_t>(32 * quarter) << 16;
+
+  if (key_cta) {
+    // ================================================================ 128 keys: dK, dV
+    const int64_t per_tile = static_cast<int64_t>(g.batch) * g.hkv * g.parts;
+    const int kt = static_cast<int>(blockIdx.x / per_tile);   // causal: the first key tiles see the most queries
+    const int64_t rest = blockIdx.x % per_tile;
+    const int part = static_cast<int>(rest % g.parts);
+    const int bh = static_cast<int>(rest / g.parts);
+    const int b = bh / g.hkv, kvh = bh % g.hkv;
+    int64_t lo, hi;
+    int first, count;
+    key_tile_queries(g, b, kt, lo, hi, first, count);
+    // this CTA's share of the (head, query tile) pairs
+    const int total = g.group * count;
+    const int chunk = (total + g.parts - 1) / g.parts;
+    const int begin = part * chunk < total ? part * chunk : total;
+    const int n = (begin + chunk < total ? begin + chunk : total) - begin;
+    uint8_t* sK = smem;
+    uint8_t* sV = smem + TILE;
+    uint8_t* sQ = smem + 2 * TILE;        // 2 stages
+    uint8_t* sO = smem + 4 * TILE;        // 2 stages
+    float* stats = reinterpret_cast<float*>(smem + 6 * TILE);   // 2 stages of [-lse | delta][128]
+    const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        Armed armed;
+        bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        for (int t = 0; t < n && ok; ++t) {
+          const int s = t & 1;
+          const uint32_t phase = (t >> 1) & 1;
+          const int head = kvh * g.group + (begin + t) / count, qt = first + (begin + t) % count;
+          auto load_q = [&]() {
+            armed.arm(bars, 2 + s, phase, TILE + 1024);
+            load_tile<NKB>(&map_q, bars + kFull + 2 + s, sQ + s * TILE, qt * AM, head, b);
+            bulk_load(stats + s * 256, g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256, 1024,
+                      bars + kFull + 2 + s);
+          };
+          auto load_do = [&]() {
+            armed.arm(bars, 4 + s, phase, TILE);
+            load_tile<NKB>(&map_do, bars + kFull + 4 + s, sO + s * TILE, qt * AM, head, b);
+          };
+          if (t == 0) {
+            armed.arm(bars, 0, 0, TILE);
+            load_tile<NKB>(&map_k, bars + kFull, sK, kt * AN, kvh, b);
+            load_q();
+            armed.arm(bars, 1, 0, TILE);
+            load_tile<NKB>(&map_v, bars + kFull + 1, sV, kt * AN, kvh, b);
+            load_do();
+            continue;
+          }
+          // the dO stage is free after dV of two tiles ago, the Q stage after its dK
+          if (!mbar_wait(bars + kEmpty + 4 + s, phase ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          load_do();
+          if (!mbar_wait(bars + kEmpty + 2 + s, phase ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          load_q();
+        }
+        if (!ok) give_up(g, abort_flag, kErrTimeoutProducer);
+        armed.wait_all(bars);   // every load of this CTA has landed before it may exit (bounded)
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0 && n > 0) {
+        auto ready = [&](int bar, uint32_t parity) -> bool {
+          if (!mbar_wait(bars + bar, parity) || *reinterpret_cast<volatile int*>(abort_flag)) return false;
+          tc_fence_after();
+          return true;
+        };
+        bool ok = stall != kErrTimeoutMma || mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        ok = ok && ready(kFull, 0) && ready(kFull + 2, 0);
+        if (ok) {
+          mma_ss<NKB>(t_s, sK, sQ, idesc_s);
+          umma_commit(bars + kS);
+          ok = ready(kFull + 1, 0) && ready(kFull + 4, 0);
+        }
+        if (ok) {
+          mma_ss<NKB>(t_dp, sV, sO, idesc_s);
+          umma_commit(bars + kDp);
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          const int s = t & 1, s1 = s ^ 1;
+          const uint32_t phase1 = ((t + 1) >> 1) & 1;
+          // P(t) written over S(t): dV, then the next S over P(t) (MMAs run in the order they are issued)
+          if (!ready(kP, t & 1)) { ok = false; break; }
+          mma_ts(t_dv, t_s, sO + s * TILE, idesc_g, t > 0);
+          umma_commit(bars + kEmpty + 4 + s);
+          if (t + 1 < n) {
+            if (!ready(kFull + 2 + s1, phase1)) { ok = false; break; }
+            mma_ss<NKB>(t_s, sK, sQ + s1 * TILE, idesc_s);
+            umma_commit(bars + kS);
+          }
+          if (!ready(kDs, t & 1)) { ok = false; break; }
+          mma_ts(t_dk, t_dp, sQ + s * TILE, idesc_g, t > 0);
+          umma_commit(bars + kEmpty + 2 + s);
+          if (t + 1 < n) {
+            if (!ready(kFull + 4 + s1, phase1)) { ok = false; break; }
+            mma_ss<NKB>(t_dp, sV, sO + s1 * TILE, idesc_s);
+            umma_commit(bars + kDp);
+          }
+        }
+        if (ok) umma_commit(bars + kDone);
+        else give_up(g, abort_flag, kErrTimeoutMma);
+      }
+      __syncwarp();
+    } else {
+      const int64_t key = static_cast<int64_t>(kt) * AN + r;
+      const bool key_seen = key >= lo && key < hi;
+      bool ok = true;
+      if (stall == kErrTimeoutEpilogue) {
+        bool waited = true;
+        if (lane == 0) waited = mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
+      }
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = t & 1;
+        const int qt = first + (begin + t) % count;
+        // first of this warp's 64 columns whose query sees the key
+        int c_lo = 64;
+        if (key_seen) {
+          const int64_t c = g.causal ? key - g.shift - static_cast<int64_t>(qt) * AM - 64 * half : 0;
+          c_lo = c < 0 ? 0 : (c > 64 ? 64 : static_cast<int>(c));
+        }
+        const bool all_seen = __all_sync(0xffffffffu, c_lo == 0);
+        // the statistics came with Q: every lane that reads them waits for their arrival itself
+        bool here = mbar_wait(bars + kFull + 2 + s, (t >> 1) & 1);
+        here = __all_sync(0xffffffffu, here);
+        if (!here || !warp_wait(bars + kS, t & 1, lane, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const float4* nl = reinterpret_cast<const float4*>(stats + s * 256 + half * 64);
+        const float4* dl = reinterpret_cast<const float4*>(stats + s * 256 + 128 + half * 64);
+        float p[64];
+        {
+          uint32_t v[64];
+          tmem_ld64(t_s + lane_addr + half * 64, v);
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const float4 m = nl[c >> 2];
+            p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, m.x));
+            p[c + 1] = fast_exp2(fmaf(__uint_as_float(v[c + 1]), g.scale_log2, m.y));
+            p[c + 2] = fast_exp2(fmaf(__uint_as_float(v[c + 2]), g.scale_log2, m.z));
+            p[c + 3] = fast_exp2(fmaf(__uint_as_float(v[c + 3]), g.scale_log2, m.w));
+          }
+        }
+        if (!all_seen) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) p[c] = c >= c_lo ? p[c] : 0.0f;
+        }
+        {
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
+          tmem_st32(t_s + lane_addr + half * 64, w);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kP);
+        if (!warp_wait(bars + kDp, t & 1, lane, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t w[32];
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t v[32];
+          tmem_ld32(t_dp + lane_addr + half * 64 + ch * 32, v);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const float4 m = dl[(ch * 32 + c) >> 2];
+            float* pp = p + ch * 32 + c;
+            pp[0] *= __uint_as_float(v[c]) - m.x;
+            pp[1] *= __uint_as_float(v[c + 1]) - m.y;
+            pp[2] *= __uint_as_float(v[c + 2]) - m.z;
+            pp[3] *= __uint_as_float(v[c + 3]) - m.w;
+          }
+        }
+        if (!all_seen) {   // a masked pair's dP may be anything (a key's V outside its range)
+#pragma unroll
+          for (int c = 0; c < 64; ++c) p[c] = c >= c_lo ? p[c] : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
+        tmem_st32(t_dp + lane_addr + half * 64, w);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kDs);
+      }
+      if (ok && n > 0) {
+        ok = warp_wait(bars + kDone, 0, lane, abort_flag);
+        tc_fence_after();
+      }
+      if (!ok) {
+        if (lane == 0) give_up(g, abort_flag, kErrTimeoutEpilogue);
+      } else if (g.parts == 1 || n > 0) {
+        // the first four warps write dV, the others c dK: one key per thread
+        const uint32_t acc = (half == 0 ? t_dv : t_dk) + lane_addr;
+        const float f = half == 0 ? 1.0f : g.scale;
+        uint16_t* out = half == 0 ? g.dv : g.dk;
+        const int64_t at = half == 0 ? b * g.dv_sb + kvh * g.dv_sh + key * g.dv_ss : b * g.dk_sb + kvh * g.dk_sh + key * g.dk_ss;
+        float* sum = g.partial + (((static_cast<int64_t>(part) * g.batch * g.hkv + bh) * g.nkt * AN + key) * 2 + half) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          if (n > 0) {
+            tmem_ld32(acc + c * 32, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
+          if (g.parts > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(sum + c * 32 + e) =
+                  make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f,
+                              __uint_as_float(v[e + 3]) * f);
+          } else if (out != nullptr && key < g.sk) {
+            store_row32<FMT>(out + at, v, f, c * 32, g.hd);
+          }
+        }
+      }
+    }
+  } else {
+    // ================================================================ 128 queries: dQ
+    const int64_t item = static_cast<int64_t>(blockIdx.x) - g.key_items;
+    const int64_t bh_count = static_cast<int64_t>(g.batch) * g.hq;
+    const int qt = g.nqt - 1 - static_cast<int>(item / bh_count);   // causal: the last query tiles see the most keys
+    const int64_t bh = item % bh_count;
+    const int b = static_cast<int>(bh / g.hq), h = static_cast<int>(bh % g.hq), kvh = h / g.group;
+    int64_t lo, hi;
+    int first, n;
+    query_tile_keys(g, b, qt, lo, hi, first, n);
+    uint8_t* sQ = smem;
+    uint8_t* sO = smem + TILE;
+    uint8_t* sK = smem + 2 * TILE;    // 3 stages
+    uint8_t* sV = smem + 5 * TILE;    // 2 stages
+    const uint32_t t_s = tmem, t_dp = tmem + 256, t_dq = tmem + 384;   // two S buffers
+
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        Armed armed;
+        bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        for (int t = 0; t < n && ok; ++t) {
+          const int sk_ = t % 3, sv_ = t & 1;
+          const uint32_t pk = (t / 3) & 1, pv = (t >> 1) & 1;
+          const int row = (first + t) * AN;
+          if (t == 0) {
+            armed.arm(bars, 0, 0, TILE);
+            load_tile<NKB>(&map_q, bars + kFull, sQ, qt * AM, h, b);
+          }
+          if (!mbar_wait(bars + kEmpty + 2 + sk_, pk ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          armed.arm(bars, 2 + sk_, pk, TILE);
+          load_tile<NKB>(&map_k, bars + kFull + 2 + sk_, sK + sk_ * TILE, row, kvh, b);
+          if (t == 0) {
+            armed.arm(bars, 1, 0, TILE);
+            load_tile<NKB>(&map_do, bars + kFull + 1, sO, qt * AM, h, b);
+          }
+          if (!mbar_wait(bars + kEmpty + 5 + sv_, pv ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          armed.arm(bars, 5 + sv_, pv, TILE);
+          load_tile<NKB>(&map_v, bars + kFull + 5 + sv_, sV + sv_ * TILE, row, kvh, b);
+        }
+        if (!ok) give_up(g, abort_flag, kErrTimeoutProducer);
+        armed.wait_all(bars);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0 && n > 0) {
+        auto ready = [&](int bar, uint32_t parity) -> bool {
+          if (!mbar_wait(bars + bar, parity) || *reinterpret_cast<volatile int*>(abort_flag)) return false;
+          tc_fence_after();
+          return true;
+        };
+        auto issue_s = [&](int t) -> bool {
+          if (!ready(kFull + 2 + t % 3, (t / 3) & 1)) return false;
+          mma_ss<NKB>(t_s + 128 * (t & 1), sQ, sK + (t % 3) * TILE, idesc_s);
+          umma_commit(bars + kS + (t & 1));
+          return true;
+        };
+        auto issue_dp = [&](int t) -> bool {
+          if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1)) return false;
+          mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
+          umma_commit(bars + kDp);
+          umma_commit(bars + kEmpty + 5 + (t & 1));
+          return true;
+        };
+        bool ok = stall != kErrTimeoutMma || mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        ok = ok && ready(kFull, 0) && issue_s(0) && ready(kFull + 1, 0) && issue_dp(0);
+        if (n > 1) ok = ok && issue_s(1);
+        for (int t = 0; t < n && ok; ++t) {
+          // dS(t) written over S(t), dP(t) read: the next dP first, for its reader waits for it soonest
+          if (!ready(kDs, t & 1)) { ok = false; break; }
+          if (t + 1 < n && !issue_dp(t + 1)) { ok = false; break; }
+          mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0);
+          umma_commit(bars + kEmpty + 2 + t % 3);
+          if (t + 2 < n && !issue_s(t + 2)) { ok = false; break; }
+        }
+        if (ok) umma_commit(bars + kDone);
+        else give_up(g, abort_flag, kErrTimeoutMma);
+      }
+      __syncwarp();
+    } else {
+      const int64_t row = static_cast<int64_t>(qt) * AM + r;
+      const bool row_in = row < g.sq;
+      const float* st = g.stats + (bh * g.nqt + qt) * 256;
+      const float nl = n > 0 ? st[r] : 0.0f, delta = n > 0 ? st[128 + r] : 0.0f;
+      int64_t end = hi;                                      // visible keys of this row: [lo, end)
+      if (g.causal && row + g.shift + 1 < end) end = row + g.shift + 1;
+      if (!row_in) end = lo;
+      bool ok = true;
+      if (stall == kErrTimeoutEpilogue) {
+        bool waited = true;
+        if (lane == 0) waited = mbar_wait(bars + kStall, 0, kStallLimitCycles);
+        ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
+      }
+      for (int t = 0; t < n && ok; ++t) {
+        const int64_t key0 = static_cast<int64_t>(first + t) * AN;
+        const int64_t a0 = lo - key0 - 64 * half, a1 = end - key0 - 64 * half;
+        const int c_lo = a0 < 0 ? 0 : (a0 > 64 ? 64 : static_cast<int>(a0));
+        const int c_hi = a1 < 0 ? 0 : (a1 > 64 ? 64 : static_cast<int>(a1));
+        const bool all_seen = __all_sync(0xffffffffu, c_lo == 0 && c_hi == 64);
+        const uint32_t my_s = t_s + 128 * (t & 1) + lane_addr + half * 64;
+        if (!warp_wait(bars + kS + (t & 1), (t >> 1) & 1, lane, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        float p[64];
+        {
+          uint32_t v[64];
+          tmem_ld64(my_s, v);
+#pragma unroll
+          for (int c = 0; c < 64; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
+        }
+        if (!warp_wait(bars + kDp, t & 1, lane, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t v[32];
+          tmem_ld32(t_dp + lane_addr + half * 64 + ch * 32, v);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) p[ch * 32 + c] *= __uint_as_float(v[c]) - delta;
+        }
+        if (!all_seen) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) p[c] = c >= c_lo && c < c_hi ? p[c] : 0.0f;
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
+        tmem_st32(my_s, w);
+        // keys outside [lo, hi) beside visible ones: their dS is 0, but 0 times a non-finite key would
+        // still reach dQ, so their K rows (S(t) has read them) are cleared
+        if (half == 0 && (lo > key0 || hi < (g.sk < key0 + AN ? g.sk : key0 + AN)) && (key0 + r < lo || key0 + r >= hi)) {
+          uint8_t* krow = sK + (t % 3) * TILE + r * 128;
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(krow + kb * SUB_BYTES + 16 * e) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kDs);
+      }
+      if (ok && n > 0) {
+        ok = warp_wait(bars + kDone, 0, lane, abort_flag);
+        tc_fence_after();
+      }
+      if (!ok) {
+        if (lane == 0) give_up(g, abort_flag, kErrTimeoutEpilogue);
+      } else {
+        uint16_t* out = g.dq + b * g.dq_sb + h * g.dq_sh + row * g.dq_ss;
+#pragma unroll 1
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+          uint32_t v[32];
+          if (n > 0) {
+            tmem_ld32(t_dq + lane_addr + c * 32, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
+          if (row_in) store_row32<FMT>(out, v, g.scale, c * 32, g.hd);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0 && *reinterpret_cast<volatile int*>(abort_flag)) {
+      // drain the MMAs an aborted CTA issued before its TMEM is released (bounded)
+      umma_commit(bars + kDrain);
+      mbar_wait(bars + kDrain, 0);
+    }
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(B_TMEM_COLS) : "memory");
+  }
+}
+
+// Per query row: -lse in log2 units (-inf for a row that sees no key, so that its probabilities are 0)
+// and delta = dO . O, in tiles of 128 rows padded with such rows. 16 lanes per row, 8 elements each.
+template <int FMT>
+__global__ void __launch_bounds__(256)
+attn_bwd_stats_kernel(const uint16_t* o, int64_t o_sb, int64_t o_sh, int64_t o_ss, const uint16_t* d, int64_t d_sb,
+                      int64_t d_sh, int64_t d_ss, const float* lse, float* stats, int hq, int64_t sq, int nqt, int hd,
+                      int64_t rows) {
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;   // row of the padded [B * Hq][nqt * 128]
+  const int l = threadIdx.x & 15;
+  if (at >= rows) return;   // whole half-warps: rows is a multiple of 128
+  const int64_t bh = at / (static_cast<int64_t>(nqt) * AM), i = at % (static_cast<int64_t>(nqt) * AM);
+  float sum = 0.0f;
+  const bool in = i < sq;
+  if (in && 8 * l < hd) {
+    const int64_t b = bh / hq, h = bh % hq;
+    float x[8], y[8];
+    load8(o, b * o_sb + h * o_sh + i * o_ss + 8 * l, FMT == 1 ? MUZO_BF16 : MUZO_F16, x);
+    load8(d, b * d_sb + h * d_sh + i * d_ss + 8 * l, FMT == 1 ? MUZO_BF16 : MUZO_F16, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+  }
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s, 16);
+  if (l == 0) {
+    const float v = in ? lse[bh * sq + i] : -INFINITY;
+    float* tile = stats + (at >> 7) * 256 + (at & 127);
+    tile[0] = v == -INFINITY ? -INFINITY : -v * kLog2e;
+    tile[128] = in ? sum : 0.0f;
+  }
+}
+
+// dK, dV of every key: the sums of its tile's parts, in order.
+template <int FMT>
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(BwdArgs g, int dpad) {
+  const int per_row = 2 * dpad / 8;
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t keys = static_cast<int64_t>(g.batch) * g.hkv * g.sk;
+  if (idx >= keys * per_row) return;
+  const int64_t row = idx / per_row;
+  const int e = static_cast<int>(idx % per_row);
+  const int which = e >= per_row / 2, c = (e % (per_row / 2)) * 8;
+  const int bh = static_cast<int>(row / g.sk);
+  const int64_t key = row % g.sk;
+  const int b = bh / g.hkv, kvh = bh % g.hkv;
+  uint16_t* out = which ? g.dk : g.dv;
+  if (out == nullptr || c >= g.hd) return;
+  int64_t lo, hi;
+  int first, count;
+  key_tile_queries(g, b, static_cast<int>(key / AN), lo, hi, first, count);
+  const int total = g.group * count;
+  const int chunk = (total + g.parts - 1) / g.parts;
+  const int used = chunk > 0 ? (total + chunk - 1) / chunk : 0;
+  float v[8] = {};
+  for (int p = 0; p < used; ++p) {
+    const float4* src = reinterpret_cast<const float4*>(
+        g.partial + (((static_cast<int64_t>(p) * g.batch * g.hkv + bh) * g.nkt * AN + key) * 2 + which) * dpad + c);
+    const float4 x = src[0], y = src[1];
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+    v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+  }
+  const int64_t at = which ? b * g.dk_sb + kvh * g.dk_sh + key * g.dk_ss : b * g.dv_sb + kvh * g.dv_sh + key * g.dv_ss;
+  *reinterpret_cast<uint4*>(out + at + c) = make_uint4(pack16<FMT>(v[0], v[1]), pack16<FMT>(v[2], v[3]),
+                                                       pack16<FMT>(v[4], v[5]), pack16<FMT>(v[6], v[7]));
+}
+
+template <int FMT, int D>
+int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
+               const BwdArgs& g, cudaStream_t s) {
+  auto kern = attn_bwd_kernel<FMT, D>;
+  static std::atomic<bool> configured[64] = {};
+  int dev = 0;
+  MUZO_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return MUZO_ERR_UNSUPPORTED;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    MUZO_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdLayout<D>::SMEM_BYTES));
+    configured[dev].store(true, std::memory_order_release);
+  }
+  kern<<<static_cast<unsigned>(g.key_items + g.query_items), B_THREADS, BwdLayout<D>::SMEM_BYTES, s>>>(mq, mk, mv, md, g);
+  int st = launch_status();
+  if (st != MUZO_OK || g.parts == 1 || g.key_items == 0) return st;
+  const int64_t threads = static_cast<int64_t>(g.batch) * g.hkv * g.sk * (2 * D / 8);
+  attn_bwd_join_kernel<FMT><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(g, D);
+  return launch_status();
+}
+
+// Parts that the (head, query tile) pairs of a key tile are divided into: enough CTAs to fill the
+// GPU where few key tiles exist, none with less than four pairs.
+int64_t key_parts(int64_t batch, int64_t hkv, int64_t group, int64_t nqt, int64_t nkt) {
+  const int64_t items = batch * hkv * nkt;
+  const int64_t pairs = group * nqt;
+  const int64_t sms = 148;
+  if (items <= 0) return 1;
+  int64_t parts = (2 * sms + items - 1) / items;
+  if (parts > pairs / 4) parts = pairs / 4;
+  if (parts > 32) parts = 32;
+  return parts < 1 ? 1 : parts;
+}
+
+int64_t stats_bytes(int64_t batch, int64_t hq, int64_t nqt) { return batch * hq * nqt * 1024; }
+
+int bwd_shape(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t hd) {
+  if (batch < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || sq < 0 || sk < 0) return MUZO_ERR_ARG;
+  if (dtype != MUZO_BF16 && dtype != MUZO_F16) return MUZO_ERR_DTYPE;
+  if (hd < 8 || hd % 8 != 0 || hd > 128) return MUZO_ERR_UNSUPPORTED;
+  if (batch > 0x7fffffffLL || hq > 0x7fffffffLL || sq > 0x7fffff00LL || sk > 0x7fffff00LL) return MUZO_ERR_UNSUPPORTED;
+  return MUZO_OK;
+}
+
+}  // namespace
+}  // namespace muzo
+
+using namespace muzo;
+
+extern "C" {
+
+int64_t muzo_attention_backward_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k,
+                                          int64_t head_dim) {
+  if (bwd_shape(dtype, batch, hq, hkv, seq_q, seq_k, head_dim) != MUZO_OK) return -1;
+  const int64_t nqt = (seq_q + AM - 1) / AM, nkt = (seq_k + AN - 1) / AN;
+  const int64_t parts = key_parts(batch, hkv, hq / hkv, nqt, nkt);
+  const int64_t sums = parts > 1 ? parts * batch * hkv * nkt * AN * 2 * (head_dim <= 64 ? 64 : 128) * 4 : 0;
+  return stats_bytes(batch, hq, nqt) + sums + 16;
+}
+
+int muzo_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                            const float* lse, void* dq, void* dk, void* dv, int dtype, int64_t batch, int64_t hq,
+                            int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim, const int64_t* strides,
+                            int causal, float scale, const int32_t* d_key_lo, const int32_t* d_key_hi,
+                            void* d_workspace, int64_t workspace_bytes, int32_t* d_status, void* stream) {
+  int st = bwd_shape(dtype, batch, hq, hkv, seq_q, seq_k, head_dim);
+  if (st != MUZO_OK) return st;
+  if (strides == nullptr || d_status == nullptr || !(scale > 0.0f && scale <= FLT_MAX)) return MUZO_ERR_ARG;
+  if (batch == 0 || (seq_q == 0 && seq_k == 0)) return MUZO_OK;
+  const bool none = seq_q == 0 || seq_k == 0;   // no pair: the gradients that exist are zero
+  if (!none && (q == nullptr || k == nullptr || v == nullptr || out == nullptr || dout == nullptr || lse == nullptr ||
+                d_workspace == nullptr))
+    return MUZO_ERR_ARG;
+  for (int i = 0; i < 24; ++i)
+    if (strides[i] % 8 != 0) return MUZO_ERR_ALIGN;
+  const void* bases[8] = {q, k, v, out, dout, dq, dk, dv};
+  for (const void* p : bases)
+    if (!aligned16p(p)) return MUZO_ERR_ALIGN;
+  if (!none && !aligned16p(d_workspace)) return MUZO_ERR_ALIGN;
+  if (!none && workspace_bytes < muzo_attention_backward_workspace(dtype, batch, hq, hkv, seq_q, seq_k, head_dim))
+    return MUZO_ERR_CAPACITY;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  BwdArgs g = {};
+  g.sq = seq_q; g.sk = seq_k; g.shift = seq_k - seq_q;
+  g.batch = static_cast<int>(batch); g.hq = static_cast<int>(hq); g.hkv = static_cast<int>(hkv);
+  g.group = static_cast<int>(hq / hkv); g.hd = static_cast<int>(head_dim); g.causal = causal ? 1 : 0;
+  g.nqt = static_cast<int>((seq_q + AM - 1) / AM);
+  g.nkt = static_cast<int>((seq_k + AN - 1) / AN);
+  g.parts = static_cast<int>(key_parts(batch, hkv, g.group, g.nqt, g.nkt));
+  g.scale = scale; g.scale_log2 = scale * kLog2e;
+  g.key_lo = d_key_lo; g.key_hi = d_key_hi;
+  g.dq = static_cast<uint16_t*>(dq); g.dk = static_cast<uint16_t*>(dk); g.dv = static_cast<uint16_t*>(dv);
+  const int64_t* t = strides + 15;
+  g.dq_sb = t[0]; g.dq_sh = t[1]; g.dq_ss = t[2];
+  g.dk_sb = t[3]; g.dk_sh = t[4]; g.dk_ss = t[5];
+  g.dv_sb = t[6]; g.dv_sh = t[7]; g.dv_ss = t[8];
+  g.status = d_status;
+  if (none) g.parts = 1;
+  g.key_items = (dk != nullptr || dv != nullptr) ? batch * hkv * g.nkt * g.parts : 0;
+  g.query_items = dq != nullptr ? batch * hq * g.nqt : 0;
+  if (g.key_items + g.query_items == 0) return MUZO_OK;
+  if (g.key_items + g.query_items > 0x7fffffffLL) return MUZO_ERR_UNSUPPORTED;
+  float* stats = static_cast<float*>(d_workspace);
+  g.stats = stats;
+  CUtensorMap mq = {}, mk = {}, mv = {}, md = {};
+  if (!none) {
+    g.partial = g.parts > 1 ? stats + stats_bytes(batch, hq, g.nqt) / 4 : nullptr;
+    st = encode_attn_map(&mq, q, dtype, head_dim, seq_q, hq, batch, strides[2], strides[1], strides[0], AM);
+    if (st != MUZO_OK) return st;
+    st = encode_attn_map(&mk, k, dtype, head_dim, seq_k, hkv, batch, strides[5], strides[4], strides[3], AN);
+    if (st != MUZO_OK) return st;
+    st = encode_attn_map(&mv, v, dtype, head_dim, seq_k, hkv, batch, strides[8], strides[7], strides[6], AN);
+    if (st != MUZO_OK) return st;
+    st = encode_attn_map(&md, dout, dtype, head_dim, seq_q, hq, batch, strides[14], strides[13], strides[12], AM);
+    if (st != MUZO_OK) return st;
+    const int64_t rows = batch * hq * g.nqt * AM;
+    const int64_t blocks = rows / 16;
+    if (blocks > 0x7fffffffLL) return MUZO_ERR_UNSUPPORTED;
+    auto pre = dtype == MUZO_BF16 ? attn_bwd_stats_kernel<1> : attn_bwd_stats_kernel<0>;
+    pre<<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const uint16_t*>(out), strides[9], strides[10], strides[11],
+                                                      static_cast<const uint16_t*>(dout), strides[12], strides[13],
+                                                      strides[14], lse, stats, g.hq, seq_q, g.nqt, g.hd, rows);
+    st = launch_status();
+    if (st != MUZO_OK) return st;
+  }
+  if (dtype == MUZO_BF16)
+    return head_dim <= 64 ? launch_bwd<1, 64>(mq, mk, mv, md, g, s) : launch_bwd<1, 128>(mq, mk, mv, md, g, s);
+  return head_dim <= 64 ? launch_bwd<0, 64>(mq, mk, mv, md, g, s) : launch_bwd<0, 128>(mq, mk, mv, md, g, s);
+}
+
+}  // extern "C"

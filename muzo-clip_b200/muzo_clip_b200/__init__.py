@@ -4,6 +4,7 @@ Drop-in for the reference package ``muzo_clip``: the same public names, signatur
 statistics, backed by the native library ``libmuzo_b200.so`` (C ABI in include/muzo_b200.h).
 """
 
+from .attention import attention_max, attention_max_backward
 from .muzo_optimizer import MuZOClipOptimizer
 from .newton_schulz import zeropower_via_newtonschulz5
 from .parameter_filter import select_muzo_parameters
@@ -12,6 +13,8 @@ from .qk_clip import use_qk_capture_attention
 
 __all__ = [
     "MuZOClipOptimizer",
+    "attention_max",
+    "attention_max_backward",
     "iter_param_blocks",
     "make_zo_noise_like",
     "select_muzo_parameters",

@@ -114,6 +114,15 @@ _SIGNATURES = {
         [_vp, _vp, _vp, _vp, _i32] + [_i64] * 6 + [_i64] * 12 + [_i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
         _i32,
     ),
+    "muzo_attention_max_lse": (
+        [_vp, _vp, _vp, _vp, _vp, _i32] + [_i64] * 6 + [_i64] * 12 + [_i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
+        _i32,
+    ),
+    "muzo_attention_backward_workspace": ([_i32] + [_i64] * 6, _i64),
+    "muzo_attention_backward": (
+        [_vp] * 9 + [_i32] + [_i64] * 6 + [_vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
+        _i32,
+    ),
     "muzo_ipc_export": ([_vp, _vp, _vp, _vp], _i32),
     "muzo_ipc_import": ([_vp, _vp], _i32),
     "muzo_ipc_close": ([_vp], _i32),
@@ -139,7 +148,8 @@ KERNELS_PER_CALL = {
     "muzo_ns_prepare": 1, "muzo_rebuild_segments_history": 1, "muzo_rebuild_kept_linear": 1,
     "muzo_ns_normalize": 1, "muzo_ns_gemm": 1, "muzo_update_sumsq": 1, "muzo_apply_update": 1,
     "muzo_qk_scale_rows": 1, "muzo_qk_max": 3, "muzo_qk_max_ranges": 3, "muzo_logits_head_max": 3, "muzo_max_merge": 1,
-    "muzo_ns_normalize_noalloc": 3, "muzo_attention_max": 3, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
+    "muzo_ns_normalize_noalloc": 3, "muzo_attention_max": 3, "muzo_attention_max_lse": 3,
+    "muzo_attention_backward_workspace": 0, "muzo_attention_backward": 2, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
     "muzo_push_blocks": 0,
 }
 launch_count = 0
@@ -181,6 +191,26 @@ def dist_code(distribution: str) -> int:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """The current device already is the one asked for."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to ``device``: the library launches on the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 _DEVICE_PROPS: dict[int, tuple[int, int]] = {}

@@ -11,6 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .attention import attention_max, attention_status, check_attention_status  # noqa: F401
 
 _ACTIVE = contextvars.ContextVar("muzo_qk_controller", default=None)
 _REGISTERED = False
@@ -230,32 +231,6 @@ def scale_rows_many(jobs: list) -> None:
 
 # ---------------------------------------------------------------- fused attention
 
-_ATTN_STATUS: dict[int, torch.Tensor] = {}
-
-
-def attention_status(device: torch.device) -> torch.Tensor:
-    """Two device int32 words per GPU: [0] the first nonzero timeout code of a fused attention
-    launch, [1] the stall request (0; tests set a role's code to make its first wait expire)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    t = _ATTN_STATUS.get(idx)
-    if t is None:
-        t = torch.zeros(2, dtype=torch.int32, device=device)
-        _ATTN_STATUS[idx] = t
-    return t
-
-
-def check_attention_status(device: torch.device) -> None:
-    """Raise if a fused attention launch on `device` reported an expired wait (reads one word)."""
-    if device.type != "cuda" or not _ATTN_STATUS:
-        return
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    t = _ATTN_STATUS.get(idx)
-    if t is not None and int(t[0].item()) != 0:
-        code = int(t[0].item())
-        t[0].zero_()
-        raise _lib.MuzoError(f"fused attention reported status {code} (a bounded wait expired); the outputs of "
-                             "the forward that ran it are unspecified")
-
 
 def fused_attention_eligible(query, key, value, dropout: float) -> bool:
     """True when the tcgen05 attention kernel can take this call: bf16/fp16 CUDA states with head
@@ -273,31 +248,6 @@ def fused_attention_eligible(query, key, value, dropout: float) -> bool:
         if t.stride(-1) != 1 or any(int(st) % 8 for st in t.stride()[:3]) or t.data_ptr() % 16:
             return False
     return True
-
-
-def attention_max(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float, causal: bool,
-                  key_lo: torch.Tensor | None = None, key_hi: torch.Tensor | None = None,
-                  record: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
-    """softmax(scaling * Q K^T) V on the tensor cores for Q [B, Hq, Sq, D], K, V [B, Hkv, Sk, D]
-    (transformers' transposed views), returned as [B, Sq, Hq, D] (the layout attention functions
-    return); with ``record``, also the per-head max of the eager pre-softmax logits and a validity
-    word, on the device. ``key_lo``/``key_hi`` (int32 per batch) bound the visible keys."""
-    b, hq, sq, d = (int(v) for v in query.shape)
-    hkv, sk = int(key.shape[1]), int(key.shape[2])
-    dev = query.device
-    out = torch.empty((b, sq, hq, d), dtype=query.dtype, device=dev)
-    smax = torch.empty(hq, dtype=torch.float32, device=dev) if record else None
-    valid = torch.empty(1, dtype=torch.int32, device=dev) if record else None
-    status = attention_status(dev)
-    _lib.launch("muzo_attention_max", query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(),
-                _lib.dtype_code(query.dtype), b, hq, hkv, sq, sk, d,
-                query.stride(0), query.stride(1), query.stride(2), key.stride(0), key.stride(1), key.stride(2),
-                value.stride(0), value.stride(1), value.stride(2), sq * hq * d, d, hq * d,
-                1 if causal else 0, float(scaling),
-                key_lo.data_ptr() if key_lo is not None else None, key_hi.data_ptr() if key_hi is not None else None,
-                smax.data_ptr() if smax is not None else None, valid.data_ptr() if valid is not None else None,
-                status.data_ptr(), _lib.stream_ptr(dev))
-    return out, smax, valid
 
 
 # ---------------------------------------------------------------- probe attention
