@@ -378,6 +378,26 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
 int muzo_qk_scale_rows(void* w, int dtype, int64_t groups, int64_t rows_per_group, int64_t cols,
                        const float* d_factors, const int32_t* d_mask, void* stream);
 
+/* ---------------------------------------------------------------- gradient norm and clipping */
+
+/* The norm over `count` tensors at once (no counterpart in the reference, which has no gradients):
+ * src, numel and dtype are host arrays of device addresses, element counts and muzo_dtype codes;
+ * types may mix, empty tensors are skipped, addresses need only their element's alignment. *d_norm
+ * (device float) = sqrt(sum g^2), summed in fp64 over fp32 partial squares, or max |g| when
+ * inf_norm != 0 (NaN if any g is NaN). Two launches for up to 1150 tensors: the tables travel as
+ * kernel parameters, so the host arrays are free again when the call returns.
+ * muzo_grad_clip also writes dst[i] = dst_dtype(g * min(1, max_norm / (norm + 1e-6))): dst_dtype[i]
+ * is src_dtype[i] or MUZO_F32, dst[i] may be src[i] (same type), and what is written must not
+ * otherwise overlap anything the call reads or writes (MUZO_ERR_ARG). A NaN norm makes every
+ * result NaN. d_workspace: muzo_grad_workspace(count, total elements) bytes of device memory,
+ * 8-byte aligned, that no other call uses until this one has finished (negative: bad arguments). */
+int64_t muzo_grad_workspace(int64_t count, int64_t elements);
+int muzo_grad_norm(const uint64_t* src, const int64_t* numel, const int32_t* dtype, int64_t count, int inf_norm,
+                   float* d_norm, void* d_workspace, int64_t workspace_bytes, void* stream);
+int muzo_grad_clip(const uint64_t* src, const uint64_t* dst, const int64_t* numel, const int32_t* src_dtype,
+                   const int32_t* dst_dtype, int64_t count, int inf_norm, float max_norm, float* d_norm,
+                   void* d_workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- weight exchange between ranks */
 
 /* The step of a data-parallel job is sharded by matrix: each rank orthogonalises and updates the

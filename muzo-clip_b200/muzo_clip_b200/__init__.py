@@ -5,6 +5,7 @@ statistics, backed by the native library ``libmuzo_b200.so`` (C ABI in include/m
 """
 
 from .attention import attention_max, attention_max_backward
+from .grad_clip import clip_grad_norm_, clip_grads, grad_norm
 from .muzo_optimizer import MuZOClipOptimizer
 from .newton_schulz import zeropower_via_newtonschulz5
 from .parameter_filter import select_muzo_parameters
@@ -15,6 +16,9 @@ __all__ = [
     "MuZOClipOptimizer",
     "attention_max",
     "attention_max_backward",
+    "clip_grad_norm_",
+    "clip_grads",
+    "grad_norm",
     "iter_param_blocks",
     "make_zo_noise_like",
     "select_muzo_parameters",

@@ -123,6 +123,9 @@ _SIGNATURES = {
         [_vp] * 9 + [_i32] + [_i64] * 6 + [_vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
         _i32,
     ),
+    "muzo_grad_workspace": ([_i64, _i64], _i64),
+    "muzo_grad_norm": ([_vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _vp], _i32),
+    "muzo_grad_clip": ([_vp, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _vp, _vp, _i64, _vp], _i32),
     "muzo_ipc_export": ([_vp, _vp, _vp, _vp], _i32),
     "muzo_ipc_import": ([_vp, _vp], _i32),
     "muzo_ipc_close": ([_vp], _i32),
@@ -149,7 +152,8 @@ KERNELS_PER_CALL = {
     "muzo_ns_normalize": 1, "muzo_ns_gemm": 1, "muzo_update_sumsq": 1, "muzo_apply_update": 1,
     "muzo_qk_scale_rows": 1, "muzo_qk_max": 3, "muzo_qk_max_ranges": 3, "muzo_logits_head_max": 3, "muzo_max_merge": 1,
     "muzo_ns_normalize_noalloc": 3, "muzo_attention_max": 3, "muzo_attention_max_lse": 3,
-    "muzo_attention_backward_workspace": 0, "muzo_attention_backward": 2, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
+    "muzo_attention_backward_workspace": 0, "muzo_attention_backward": 2,
+    "muzo_grad_workspace": 0, "muzo_grad_norm": 2, "muzo_grad_clip": 2, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
     "muzo_push_blocks": 0,
 }
 launch_count = 0

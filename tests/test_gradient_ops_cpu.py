@@ -89,3 +89,64 @@ def test_readable_layouts():
               torch.zeros((2, 3, 64, 5), dtype=torch.bfloat16).transpose(2, 3)):
         copy, strides = _readable(t)
         assert copy.is_contiguous() and torch.equal(copy, t) and not any(s % 8 or s == 0 for s in strides)
+
+
+def _u64(*v):
+    return (ctypes.c_uint64 * len(v))(*v)
+
+
+def _i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def _i32(*v):
+    return (ctypes.c_int32 * len(v))(*v)
+
+
+@pytest.mark.parametrize("change, expected", [
+    ({"src": None}, 1), ({"num": None}, 1), ({"kind": None}, 1), ({"norm": None}, 1), ({"ws": None}, 1), ({"n": -1}, 1),
+    ({"num": _i64(-1)}, 1), ({"src": _u64(0)}, 1), ({"kind": _i32(7)}, 2), ({"src": _u64(257)}, 3),
+    ({"src": _u64(258), "kind": _i32(0)}, 3), ({"ws": _P + 4}, 3), ({"size": 64}, 5), ({"num": _i64(1 << 41)}, 6),
+])
+def test_norm_refuses_before_any_launch(change, expected):
+    from muzo_clip_b200 import _lib
+
+    a = {"src": _u64(256), "num": _i64(64), "kind": _i32(1), "n": 1, "norm": _P, "ws": _P, "size": 1 << 30, **change}
+    assert _lib.lib.muzo_grad_norm(a["src"], a["num"], a["kind"], a["n"], 0, a["norm"], a["ws"], a["size"], None) == expected
+
+
+@pytest.mark.parametrize("change, expected", [
+    ({"dst": None}, 1), ({"to": None}, 1), ({"to": _i32(2, 1)}, 2), ({"max": -1.0}, 1), ({"max": float("nan")}, 1),
+    ({"dst": _u64(1024, 1024)}, 1),                                  # two results in one place
+    ({"dst": _u64(256 + 64, 4096)}, 1),                              # a result over another element of its own source
+    ({"dst": _u64(256, 300)}, 1),                                    # a result over another tensor's source
+    ({"dst": _u64(0, 512)}, 1),
+    ({"to": _i32(0, 1)}, 1),                                         # in place, but wider
+    ({"size": 64}, 5),                                               # separate results pass the overlap check
+    ({"dst": _u64(2048, 4096), "size": 64}, 5),
+])
+def test_clip_refuses_before_any_launch(change, expected):
+    from muzo_clip_b200 import _lib
+
+    a = {"src": _u64(256, 512), "dst": _u64(256, 512), "num": _i64(64, 64), "kind": _i32(1, 1), "to": _i32(1, 1), "max": 1.0,
+         "size": 1 << 30, **change}
+    assert _lib.lib.muzo_grad_clip(a["src"], a["dst"], a["num"], a["kind"], a["to"], 2, 0, a["max"], _P, _P, a["size"],
+                                   None) == expected
+
+
+def test_flat_layouts():
+    from muzo_clip_b200.grad_clip import _flat
+
+    t = torch.zeros(4, 6, 8)
+    assert _flat(t) and _flat(t.transpose(0, 2)) and _flat(t[1:3]) and _flat(t[:, :1, :1][:1]) and _flat(torch.zeros(0, 3))
+    assert not _flat(t[:, 1:3]) and not _flat(t[..., ::2]) and not _flat(torch.zeros(1).expand(5))
+
+
+def test_gradient_functions_refuse_cpu_tensors():
+    from muzo_clip_b200 import clip_grads, grad_norm
+
+    with pytest.raises(ValueError):
+        grad_norm([torch.zeros(4)])
+    with pytest.raises(ValueError):
+        clip_grads([torch.zeros(4)], 1.0)
+    assert float(grad_norm([])) == 0.0
