@@ -310,14 +310,47 @@ def ensure_probe_registered() -> str:
     return PROBE_ATTENTION
 
 
+def _fused_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
+    """Attention function of fused training: ``attention_max`` computes the output, its gradients
+    and, while a QK-Clip capture is active, the per-head maxima in the same kernel. It takes no
+    mask, the causal mask and padding masks (as key ranges) over bf16/fp16 states; what it does not
+    take (dropout, other masks, fp32, other head dimensions, a causal call without a mask whose
+    queries and keys differ in number) goes to the capture attention on SDPA."""
+    mask = attention_mask if attention_mask is not None and attention_mask.ndim == 4 else None
+    sq, sk = query.shape[2], key.shape[2]
+    causal = kwargs.get("is_causal")
+    causal = (bool(getattr(module, "is_causal", True)) if causal is None else bool(causal)) and sq > 1
+    lo = hi = None
+    ok = (not dropout and query.is_cuda and query.dtype in (torch.bfloat16, torch.float16)
+          and key.dtype == query.dtype and value.dtype == query.dtype and key.shape == value.shape
+          and query.shape[-1] == key.shape[-1] <= 128 and query.shape[-1] % 8 == 0
+          and query.shape[1] % key.shape[1] == 0 and (scaling is None or scaling > 0.0)
+          and (attention_mask is None or mask is not None))
+    if ok and mask is not None:
+        ranges = mask_key_ranges(mask, query.shape[0], sq, sk)
+        ok = ranges is not None
+        if ok:
+            causal, lo, hi = ranges
+    elif ok:
+        ok = not causal or sq == sk
+    if not ok:
+        return _probe_attention(module, query, key, value, attention_mask, scaling=scaling, dropout=dropout, **kwargs)
+    ctrl = _ACTIVE.get()
+    name = ctrl.module_name(module) if ctrl is not None else None
+    out, smax, valid = attention_max(query, key, value, scaling, causal, lo, hi, record=name is not None)
+    if name is not None:
+        ctrl.record_max(name, smax, valid)
+    return out, None
+
+
 _TRAINING_REGISTERED = False
 
 
-def ensure_training_registered() -> str:
-    """Register the training-time capture attention with SDPA's mask format (no mask for plain
-    causal attention, so SDPA keeps its fused causal kernels) once."""
+def ensure_training_registered(fused: bool = False) -> str:
+    """Register the training-time capture attentions (on SDPA, and fused) with SDPA's mask format
+    (no mask for plain causal attention, so SDPA keeps its fused causal kernels) once."""
     global _TRAINING_REGISTERED
-    from .qk_clip import CAPTURE_ATTENTION
+    from .qk_clip import CAPTURE_ATTENTION, FUSED_ATTENTION
 
     if not _TRAINING_REGISTERED:
         from transformers import AttentionInterface
@@ -325,5 +358,7 @@ def ensure_training_registered() -> str:
 
         AttentionInterface.register(CAPTURE_ATTENTION, _probe_attention)
         ALL_MASK_ATTENTION_FUNCTIONS.register(CAPTURE_ATTENTION, sdpa_mask)
+        AttentionInterface.register(FUSED_ATTENTION, _fused_attention)
+        ALL_MASK_ATTENTION_FUNCTIONS.register(FUSED_ATTENTION, sdpa_mask)
         _TRAINING_REGISTERED = True
-    return CAPTURE_ATTENTION
+    return FUSED_ATTENTION if fused else CAPTURE_ATTENTION

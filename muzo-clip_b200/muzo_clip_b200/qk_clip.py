@@ -35,16 +35,19 @@ logger = logging.getLogger(__name__)
 
 PROBE_ATTENTION = "muzo_qk_probe"
 CAPTURE_ATTENTION = "muzo_qk_sdpa"
+FUSED_ATTENTION = "muzo_qk_fused"
 
 
-def use_qk_capture_attention(model: torch.nn.Module) -> str:
+def use_qk_capture_attention(model: torch.nn.Module, fused: bool = False) -> str:
     """Make ``model`` (a transformers model) train with the QK-capture attention: SDPA for the
     output and gradients, plus the library's max-logit kernel on the same query/key states
     while a QK-Clip capture is active — e.g. the clean forward of
     ``MuZOClipOptimizer(..., enable_qk_clip=True, qk_capture_clean_forward=True)`` — so exact
     per-head maxima are collected without eager attention and without a separate probe. Outside
-    a capture the attention is SDPA alone. Returns the implementation name."""
-    impl = _qk.ensure_training_registered()
+    a capture the attention is SDPA alone. With ``fused=True`` the library's own attention kernels
+    compute the output, the gradients and the maxima together (``attention_max``; calls they do not
+    take go to SDPA as above). Returns the implementation name."""
+    impl = _qk.ensure_training_registered(fused)
     seen: list[Any] = []
     for module in model.modules():
         config = getattr(module, "config", None)
