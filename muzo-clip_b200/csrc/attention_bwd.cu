@@ -25,8 +25,8 @@ namespace {
 using namespace tc;
 using namespace attn;
 
-constexpr int B_THREADS = 320;   // warp 0 TMA, warp 1 MMA, warps 2..9 probabilities: two warps per TMEM
-                                 // lane quarter, 64 of the tile's 128 columns each
+constexpr int B_THREADS = 352;   // warp 0 TMA, warps 1 and 10 MMA, warps 2..9 probabilities: two warps per
+                                 // TMEM lane quarter, 64 of the tile's 128 columns each
 constexpr uint32_t B_TMEM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -34,9 +34,10 @@ template <int D>
 struct BwdLayout {
   static constexpr int NKB = D / ABK;
   static constexpr int TILE_BYTES = NKB * SUB_BYTES;   // 128 rows of one operand
-  static constexpr int TILES = 7;                      // key CTA: K, V, 2 Q, 2 dO, statistics; query CTA: Q, dO, 3 K, 2 V
+  static constexpr int TILES = 7;                      // key CTA: K, V, 3 Q, 2 dO; query CTA: Q, dO, 3 K, 2 V
+  static constexpr int STAT_BYTES = 5 * 512;           // key CTA: delta with each Q stage, -lse with each dO stage
   static constexpr int BAR_BYTES = 256;
-  static constexpr int NEED = TILES * TILE_BYTES + BAR_BYTES + 1024;
+  static constexpr int NEED = TILES * TILE_BYTES + STAT_BYTES + BAR_BYTES;
   static constexpr int SMEM_BYTES = NEED > 116 * 1024 ? NEED : 116 * 1024;   // one CTA per SM: it takes all of TMEM
 };
 
@@ -78,10 +79,35 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return FMT == 1 ? pack_bf16(lo, hi) : pack_half(lo, hi);
 }
 
-// One lane waits for the barrier, the warp shares the answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int lane, const int* abort_flag) {
+// Bounded waits of one thread and of a warp (one lane polls, all get its answer). A phase that is
+// complete costs one poll; the abort flag and the clock are read between polls only. The waits on the
+// path between the tensor cores and the probabilities poll with test_wait: a thread that try_wait
+// has suspended wakes 250 to 650 cycles after the phase, in one of eight warps or the other.
+__device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+template <bool SPIN = true>
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  if (SPIN ? poll(addr, parity) : mbar_try_wait(addr, parity)) return true;
+  const long long start = clock64();
+  while (!(SPIN ? poll(addr, parity) : mbar_try_wait(addr, parity))) {
+    if (*reinterpret_cast<const volatile int*>(abort_flag)) return false;
+    if (static_cast<unsigned long long>(clock64() - start) > kWaitLimitCycles) return false;
+  }
+  return true;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const int* abort_flag) {
   bool ready = true;
-  if (lane == 0) ready = mbar_wait(bar, parity) && !*reinterpret_cast<const volatile int*>(abort_flag);
+  if ((threadIdx.x & 31) == 0) ready = wait_one(bar, parity, abort_flag);
   return __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
 }
 
@@ -133,16 +159,16 @@ __device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[3
 
 // Barriers of both kinds of CTA.
 enum : int {
-  kFull = 0,        // key CTA: K, V, Q[2], dO[2]; query CTA: Q, dO, K[3], V[2]
-  kEmpty = 7,       // key CTA: Q[2], dO[2] (at 2 and 4); query CTA: K[3], V[2] (at 2 and 5)
+  kFull = 0,        // key CTA: K, V, Q[3], dO[2]; query CTA: Q, dO, K[3], V[2]
+  kEmpty = 7,       // key CTA: Q[3], dO[2] (at 2 and 5); query CTA: K[3], V[2] (at 2 and 5)
   kS = 14,          // S computed (query CTA: two, by buffer)
   kDp = 16,         // dP computed
-  kP = 17,          // key CTA: P written and S read
-  kDs = 18,         // dS written and dP read
-  kDone = 19,
-  kDrain = 20,
-  kStall = 21,
-  kBars = 22
+  kP = 17,          // key CTA: P written, S read, the next tile's loads here
+  kDs = 18,         // dS written and dP read (query CTA: two, by buffer: its two readers run apart)
+  kDone = 20,
+  kDrain = 21,      // two: one per issuer
+  kStall = 23,
+  kBars = 24
 };
 
 // Loads issued by the producer thread: which full barriers are armed, and with which parity.
@@ -200,9 +226,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   using L = BwdLayout<D>;
   constexpr int NKB = L::NKB;
   constexpr int TILE = L::TILE_BYTES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::TILES * TILE);
+  extern __shared__ __align__(1024) uint8_t smem[];   // 1024: the swizzled tiles' alignment
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::TILES * TILE + L::STAT_BYTES);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kBars);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
 
@@ -211,7 +236,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBars; ++i) mbar_init(bars + i, (i == kP || i == kDs) ? 8 : 1);
+    // eight warps arrive on kP (with the one that waits for the loads) and kDs, a query CTA's two issuers on kDone
+    for (int i = 0; i < kBars; ++i)
+      mbar_init(bars + i, i == kP ? 9 : (i == kDs || i == kDs + 1 ? 8 : (i == kDone && !key_cta ? 2 : 1)));
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -249,9 +276,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int n = (begin + chunk < total ? begin + chunk : total) - begin;
     uint8_t* sK = smem;
     uint8_t* sV = smem + TILE;
-    uint8_t* sQ = smem + 2 * TILE;        // 2 stages
-    uint8_t* sO = smem + 4 * TILE;        // 2 stages
-    float* stats = reinterpret_cast<float*>(smem + 6 * TILE);   // 2 stages of [-lse | delta][128]
+    uint8_t* sQ = smem + 2 * TILE;        // 3 stages
+    uint8_t* sO = smem + 5 * TILE;        // 2 stages
+    float* delta = reinterpret_cast<float*>(smem + L::TILES * TILE);   // [3][128], with Q
+    float* neg_lse = delta + 3 * 128;                                  // [2][128], with dO
     const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
 
     if (warp == 0) {
@@ -259,42 +287,36 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         Armed armed;
         bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
         for (int t = 0; t < n && ok; ++t) {
-          const int s = t & 1;
-          const uint32_t phase = (t >> 1) & 1;
+          const int sq = t % 3, so = t & 1;
+          const uint32_t pq = (t / 3) & 1, po = (t >> 1) & 1;
           const int head = kvh * g.group + (begin + t) / count, qt = first + (begin + t) % count;
-          auto load_q = [&]() {
-            armed.arm(bars, 2 + s, phase, TILE + 1024);
-            load_tile<NKB>(&map_q, bars + kFull + 2 + s, sQ + s * TILE, qt * AM, head, b);
-            bulk_load(stats + s * 256, g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256, 1024,
-                      bars + kFull + 2 + s);
-          };
-          auto load_do = [&]() {
-            armed.arm(bars, 4 + s, phase, TILE);
-            load_tile<NKB>(&map_do, bars + kFull + 4 + s, sO + s * TILE, qt * AM, head, b);
-          };
+          const float* st = g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256;
           if (t == 0) {
             armed.arm(bars, 0, 0, TILE);
             load_tile<NKB>(&map_k, bars + kFull, sK, kt * AN, kvh, b);
-            load_q();
+          }
+          // a Q stage is free after its dK, a dO stage after its dV (issued behind dP)
+          if (!wait_one<false>(bars + kEmpty + 2 + sq, pq ^ 1, abort_flag)) { ok = false; break; }
+          armed.arm(bars, 2 + sq, pq, TILE + 512);
+          load_tile<NKB>(&map_q, bars + kFull + 2 + sq, sQ + sq * TILE, qt * AM, head, b);
+          bulk_load(delta + sq * 128, st + 128, 512, bars + kFull + 2 + sq);
+          if (t == 0) {
             armed.arm(bars, 1, 0, TILE);
             load_tile<NKB>(&map_v, bars + kFull + 1, sV, kt * AN, kvh, b);
-            load_do();
-            continue;
           }
-          // the dO stage is free after dV of two tiles ago, the Q stage after its dK
-          if (!mbar_wait(bars + kEmpty + 4 + s, phase ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
-          load_do();
-          if (!mbar_wait(bars + kEmpty + 2 + s, phase ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
-          load_q();
+          if (!wait_one<false>(bars + kEmpty + 5 + so, po ^ 1, abort_flag)) { ok = false; break; }
+          armed.arm(bars, 5 + so, po, TILE + 512);
+          bulk_load(neg_lse + so * 128, st, 512, bars + kFull + 5 + so);
+          load_tile<NKB>(&map_do, bars + kFull + 5 + so, sO + so * TILE, qt * AM, head, b);
         }
         if (!ok) give_up(g, abort_flag, kErrTimeoutProducer);
         armed.wait_all(bars);   // every load of this CTA has landed before it may exit (bounded)
       }
       __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0 && n > 0) {
+      if (n > 0 && elect_one()) {
         auto ready = [&](int bar, uint32_t parity) -> bool {
-          if (!mbar_wait(bars + bar, parity) || *reinterpret_cast<volatile int*>(abort_flag)) return false;
+          if (!wait_one(bars + bar, parity, abort_flag)) return false;
           tc_fence_after();
           return true;
         };
@@ -303,35 +325,48 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (ok) {
           mma_ss<NKB>(t_s, sK, sQ, idesc_s);
           umma_commit(bars + kS);
-          ok = ready(kFull + 1, 0) && ready(kFull + 4, 0);
+          ok = ready(kFull + 1, 0) && ready(kFull + 5, 0);
         }
         if (ok) {
           mma_ss<NKB>(t_dp, sV, sO, idesc_s);
           umma_commit(bars + kDp);
         }
         for (int t = 0; t < n && ok; ++t) {
-          const int s = t & 1, s1 = s ^ 1;
-          const uint32_t phase1 = ((t + 1) >> 1) & 1;
-          // P(t) written over S(t): dV, then the next S over P(t) (MMAs run in the order they are issued)
+          const int so = t & 1;
+          // P(t) written over S(t), the next Q and dO loaded (warp 10 arrives for them): dV, then the next S
+          // over P(t) (MMAs run in the order they are issued)
           if (!ready(kP, t & 1)) { ok = false; break; }
-          mma_ts(t_dv, t_s, sO + s * TILE, idesc_g, t > 0);
-          umma_commit(bars + kEmpty + 4 + s);
+          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, t > 0);
+          umma_commit(bars + kEmpty + 5 + so);
           if (t + 1 < n) {
-            if (!ready(kFull + 2 + s1, phase1)) { ok = false; break; }
-            mma_ss<NKB>(t_s, sK, sQ + s1 * TILE, idesc_s);
+            mma_ss<NKB>(t_s, sK, sQ + ((t + 1) % 3) * TILE, idesc_s);
             umma_commit(bars + kS);
           }
           if (!ready(kDs, t & 1)) { ok = false; break; }
-          mma_ts(t_dk, t_dp, sQ + s * TILE, idesc_g, t > 0);
-          umma_commit(bars + kEmpty + 2 + s);
+          mma_ts(t_dk, t_dp, sQ + (t % 3) * TILE, idesc_g, t > 0);
+          umma_commit(bars + kEmpty + 2 + t % 3);
           if (t + 1 < n) {
-            if (!ready(kFull + 4 + s1, phase1)) { ok = false; break; }
-            mma_ss<NKB>(t_dp, sV, sO + s1 * TILE, idesc_s);
+            mma_ss<NKB>(t_dp, sV, sO + (so ^ 1) * TILE, idesc_s);
             umma_commit(bars + kDp);
           }
         }
         if (ok) umma_commit(bars + kDone);
         else give_up(g, abort_flag, kErrTimeoutMma);
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // Waits for the loads in the issuer's place: its polls queue behind the MMAs it has issued (150 to
+      // 270 cycles each, with the tensor cores idle), so it is left with two per tile.
+      if (lane == 0 && n > 0) {
+        bool ok = true;
+        for (int t = 0; t < n && ok; ++t) {
+          if (t > 0) ok = wait_one<false>(bars + kP, (t - 1) & 1, abort_flag);
+          if (ok && t + 1 < n)
+            ok = wait_one<false>(bars + kFull + 2 + (t + 1) % 3, ((t + 1) / 3) & 1, abort_flag) &&
+                 wait_one<false>(bars + kFull + 5 + ((t + 1) & 1), ((t + 1) >> 1) & 1, abort_flag);
+          if (ok) mbar_arrive(bars + kP);
+        }
+        if (!ok) give_up(g, abort_flag, kErrTimeoutMma);
       }
       __syncwarp();
     } else {
@@ -344,7 +379,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
       }
       for (int t = 0; t < n && ok; ++t) {
-        const int s = t & 1;
+        const int sq = t % 3, so = t & 1;
         const int qt = first + (begin + t) % count;
         // first of this warp's 64 columns whose query sees the key
         int c_lo = 64;
@@ -353,13 +388,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           c_lo = c < 0 ? 0 : (c > 64 ? 64 : static_cast<int>(c));
         }
         const bool all_seen = __all_sync(0xffffffffu, c_lo == 0);
-        // the statistics came with Q: every lane that reads them waits for their arrival itself
-        bool here = mbar_wait(bars + kFull + 2 + s, (t >> 1) & 1);
-        here = __all_sync(0xffffffffu, here);
-        if (!here || !warp_wait(bars + kS, t & 1, lane, abort_flag)) { ok = false; break; }
+        // the statistics came with Q and dO: their readers wait for those barriers too
+        if (!warp_wait(bars + kFull + 5 + so, (t >> 1) & 1, abort_flag) ||
+            !warp_wait(bars + kFull + 2 + sq, (t / 3) & 1, abort_flag) || !warp_wait(bars + kS, t & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
-        const float4* nl = reinterpret_cast<const float4*>(stats + s * 256 + half * 64);
-        const float4* dl = reinterpret_cast<const float4*>(stats + s * 256 + 128 + half * 64);
+        const float4* nl = reinterpret_cast<const float4*>(neg_lse + so * 128 + half * 64);
+        const float4* dl = reinterpret_cast<const float4*>(delta + sq * 128 + half * 64);
         float p[64];
         {
           uint32_t v[64];
@@ -386,7 +423,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kP);
-        if (!warp_wait(bars + kDp, t & 1, lane, abort_flag)) { ok = false; break; }
+        if (!warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         uint32_t w[32];
 #pragma unroll
@@ -415,7 +452,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (lane == 0) mbar_arrive(bars + kDs);
       }
       if (ok && n > 0) {
-        ok = warp_wait(bars + kDone, 0, lane, abort_flag);
+        ok = warp_wait(bars + kDone, 0, abort_flag);
         tc_fence_after();
       }
       if (!ok) {
@@ -476,14 +513,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             armed.arm(bars, 0, 0, TILE);
             load_tile<NKB>(&map_q, bars + kFull, sQ, qt * AM, h, b);
           }
-          if (!mbar_wait(bars + kEmpty + 2 + sk_, pk ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          if (!wait_one<false>(bars + kEmpty + 2 + sk_, pk ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 2 + sk_, pk, TILE);
           load_tile<NKB>(&map_k, bars + kFull + 2 + sk_, sK + sk_ * TILE, row, kvh, b);
           if (t == 0) {
             armed.arm(bars, 1, 0, TILE);
             load_tile<NKB>(&map_do, bars + kFull + 1, sO, qt * AM, h, b);
           }
-          if (!mbar_wait(bars + kEmpty + 5 + sv_, pv ^ 1) || *reinterpret_cast<volatile int*>(abort_flag)) { ok = false; break; }
+          if (!wait_one<false>(bars + kEmpty + 5 + sv_, pv ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 5 + sv_, pv, TILE);
           load_tile<NKB>(&map_v, bars + kFull + 5 + sv_, sV + sv_ * TILE, row, kvh, b);
         }
@@ -491,36 +528,41 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         armed.wait_all(bars);
       }
       __syncwarp();
-    } else if (warp == 1) {
-      if (lane == 0 && n > 0) {
+    } else if (warp == 1 || warp == 10) {
+      // Two issuers: warp 1 dQ(t), S(t+2) into the buffer of dS(t); warp 10 dP(t+1) once dP(t) is read.
+      if (n > 0 && elect_one()) {
         auto ready = [&](int bar, uint32_t parity) -> bool {
-          if (!mbar_wait(bars + bar, parity) || *reinterpret_cast<volatile int*>(abort_flag)) return false;
+          if (!wait_one(bars + bar, parity, abort_flag)) return false;
           tc_fence_after();
           return true;
         };
-        auto issue_s = [&](int t) -> bool {
-          if (!ready(kFull + 2 + t % 3, (t / 3) & 1)) return false;
-          mma_ss<NKB>(t_s + 128 * (t & 1), sQ, sK + (t % 3) * TILE, idesc_s);
-          umma_commit(bars + kS + (t & 1));
-          return true;
-        };
-        auto issue_dp = [&](int t) -> bool {
-          if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1)) return false;
-          mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
-          umma_commit(bars + kDp);
-          umma_commit(bars + kEmpty + 5 + (t & 1));
-          return true;
-        };
         bool ok = stall != kErrTimeoutMma || mbar_wait(bars + kStall, 0, kStallLimitCycles);
-        ok = ok && ready(kFull, 0) && issue_s(0) && ready(kFull + 1, 0) && issue_dp(0);
-        if (n > 1) ok = ok && issue_s(1);
-        for (int t = 0; t < n && ok; ++t) {
-          // dS(t) written over S(t), dP(t) read: the next dP first, for its reader waits for it soonest
-          if (!ready(kDs, t & 1)) { ok = false; break; }
-          if (t + 1 < n && !issue_dp(t + 1)) { ok = false; break; }
-          mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0);
-          umma_commit(bars + kEmpty + 2 + t % 3);
-          if (t + 2 < n && !issue_s(t + 2)) { ok = false; break; }
+        if (warp == 1) {
+          auto issue_s = [&](int t) {
+            mma_ss<NKB>(t_s + 128 * (t & 1), sQ, sK + (t % 3) * TILE, idesc_s);
+            umma_commit(bars + kS + (t & 1));
+          };
+          ok = ok && ready(kFull, 0) && ready(kFull + 2, 0);
+          if (ok) issue_s(0);
+          if (ok && n > 1) {
+            ok = ready(kFull + 3, 0);
+            if (ok) issue_s(1);
+          }
+          for (int t = 0; t < n && ok; ++t) {
+            if (t + 2 < n && !ready(kFull + 2 + (t + 2) % 3, ((t + 2) / 3) & 1)) { ok = false; break; }
+            if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
+            mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0);
+            umma_commit(bars + kEmpty + 2 + t % 3);
+            if (t + 2 < n) issue_s(t + 2);
+          }
+        } else {
+          ok = ok && ready(kFull + 1, 0);
+          for (int t = 0; t < n && ok; ++t) {
+            if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1) || (t > 0 && !ready(kDs + ((t - 1) & 1), ((t - 1) >> 1) & 1))) { ok = false; break; }
+            mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
+            umma_commit(bars + kDp);
+            umma_commit(bars + kEmpty + 5 + (t & 1));
+          }
         }
         if (ok) umma_commit(bars + kDone);
         else give_up(g, abort_flag, kErrTimeoutMma);
@@ -547,7 +589,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int c_hi = a1 < 0 ? 0 : (a1 > 64 ? 64 : static_cast<int>(a1));
         const bool all_seen = __all_sync(0xffffffffu, c_lo == 0 && c_hi == 64);
         const uint32_t my_s = t_s + 128 * (t & 1) + lane_addr + half * 64;
-        if (!warp_wait(bars + kS + (t & 1), (t >> 1) & 1, lane, abort_flag)) { ok = false; break; }
+        if (!warp_wait(bars + kS + (t & 1), (t >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         float p[64];
         {
@@ -556,7 +598,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
           for (int c = 0; c < 64; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
         }
-        if (!warp_wait(bars + kDp, t & 1, lane, abort_flag)) { ok = false; break; }
+        if (!warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
@@ -585,10 +627,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kDs);
+        if (lane == 0) mbar_arrive(bars + kDs + (t & 1));
       }
       if (ok && n > 0) {
-        ok = warp_wait(bars + kDone, 0, lane, abort_flag);
+        ok = warp_wait(bars + kDone, 0, abort_flag);
         tc_fence_after();
       }
       if (!ok) {
@@ -612,13 +654,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    if (lane == 0 && *reinterpret_cast<volatile int*>(abort_flag)) {
-      // drain the MMAs an aborted CTA issued before its TMEM is released (bounded)
-      umma_commit(bars + kDrain);
-      mbar_wait(bars + kDrain, 0);
+  if (*reinterpret_cast<volatile int*>(abort_flag)) {   // every role has ended: the same answer in all threads
+    // the MMAs that an aborted CTA issued end before its TMEM is released (bounded)
+    if ((warp == 1 || warp == 10) && elect_one()) {
+      uint64_t* drained = bars + kDrain + (warp == 1 ? 0 : 1);
+      umma_commit(drained);
+      mbar_wait(drained, 0);
     }
-    __syncwarp();
+    __syncthreads();
+  }
+  if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(B_TMEM_COLS) : "memory");
   }
