@@ -25,8 +25,8 @@ namespace {
 using namespace tc;
 using namespace attn;
 
-constexpr int B_THREADS = 352;   // warp 0 TMA, warps 1 and 10 MMA, warps 2..9 probabilities: two warps per
-                                 // TMEM lane quarter, 64 of the tile's 128 columns each
+constexpr int B_THREADS = 384;   // warp 0 TMA, warps 1 and 2 MMA, warps 4..11 probabilities: two groups of
+                                 // four, one warp of each per TMEM lane quarter
 constexpr uint32_t B_TMEM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -105,10 +105,31 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const i
   }
   return true;
 }
+// A look at a barrier ahead of time, without a branch: lane 0 polls, the answer is used later by
+// `looked_or_wait`. A poll queues behind the exponentials of both warps of a scheduler (300 cycles and
+// more), which pass meanwhile.
+__device__ __forceinline__ uint32_t look(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.eq.u32 q, %3, 0;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@q mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@q selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(threadIdx.x & 31)
+      : "memory");
+  return done;
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const int* abort_flag) {
   bool ready = true;
   if ((threadIdx.x & 31) == 0) ready = wait_one(bar, parity, abort_flag);
   return __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
+}
+
+__device__ __forceinline__ bool looked_or_wait(uint32_t looked, uint64_t* bar, uint32_t parity, const int* abort_flag) {
+  if (__shfl_sync(0xffffffffu, looked, 0) != 0) return true;
+  return warp_wait(bar, parity, abort_flag);
 }
 
 // Query tiles [first, first + count) that see a key of key tile kt in batch row b.
@@ -163,12 +184,13 @@ enum : int {
   kEmpty = 7,       // key CTA: Q[3], dO[2] (at 2 and 5); query CTA: K[3], V[2] (at 2 and 5)
   kS = 14,          // S computed (query CTA: two, by buffer)
   kDp = 16,         // dP computed
-  kP = 17,          // key CTA: P written, S read, the next tile's loads here
-  kDs = 18,         // dS written and dP read (query CTA: two, by buffer: its two readers run apart)
-  kDone = 20,
-  kDrain = 21,      // two: one per issuer
-  kStall = 23,
-  kBars = 24
+  kP = 17,          // key CTA: P written, S read, by halves of each warp's columns; with the second half, the
+                    // next tile's loads are here. Query CTA, the first: dP read
+  kDs = 19,         // dS written, and in a key CTA dP read (query CTA: two, by buffer: its readers run apart)
+  kDone = 21,
+  kDrain = 22,      // two: one per issuer
+  kStall = 24,
+  kBars = 25
 };
 
 // Loads issued by the producer thread: which full barriers are armed, and with which parity.
@@ -203,14 +225,18 @@ __device__ __forceinline__ void mma_ss(uint32_t tmem_d, const uint8_t* a, const 
                idesc, (kb > 0 || k > 0) ? 1u : 0u);
 }
 
-// D (128 x NKB*64) (+)= A B: A packed in TMEM (columns 0..31 for K rows 0..63, 64..95 for 64..127),
-// B a tile of 128 rows in shared memory read MN-major.
-__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const uint8_t* b, uint32_t idesc, bool accumulate) {
+// D (128 x NKB*64) (+)= A B: A packed in TMEM (K rows 0..63 in columns 0..31, K rows 64..127 from column
+// `second` on), B a tile of 128 rows in shared memory read MN-major. `part` 0 takes the K rows 0..31
+// and 64..95, 1 the others, 2 all.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const uint8_t* b, uint32_t idesc, bool accumulate,
+                                       int second, int part = 2) {
   const uint32_t sb = smem_u32(b);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    umma_f16_ts(tmem_d, tmem_a + (k < 4 ? 8 * k : 32 + 8 * k), make_sdesc(sb + k * (16 * 128), SUB_BYTES, 1024), idesc,
-                (accumulate || k > 0) ? 1u : 0u);
+  for (int k = 0; k < 8; ++k) {
+    if (part == 1 - ((k >> 1) & 1)) continue;
+    umma_f16_ts(tmem_d, tmem_a + (k < 4 ? 8 * k : second + 8 * (k - 4)), make_sdesc(sb + k * (16 * 128), SUB_BYTES, 1024), idesc,
+                (accumulate || k > (part == 1 ? 2 : 0) || part == 1) ? 1u : 0u);
+  }
 }
 
 // What a role that gave up does: the first code stays in the status word.
@@ -236,9 +262,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
 
   if (threadIdx.x == 0) {
-    // eight warps arrive on kP (with the one that waits for the loads) and kDs, a query CTA's two issuers on kDone
+    // arrivals: the eight probability warps on kP and kDs, the warp that waits for a key CTA's loads on its second
+    // kP, a query CTA's two issuers on kDone
     for (int i = 0; i < kBars; ++i)
-      mbar_init(bars + i, i == kP ? 9 : (i == kDs || i == kDs + 1 ? 8 : (i == kDone && !key_cta ? 2 : 1)));
+      mbar_init(bars + i, i == kP + 1 ? 9 : (i >= kP && i < kDone ? 8 : (i == kDone && !key_cta ? 2 : 1)));
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -254,7 +281,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const uint32_t tmem = *tmem_holder;
   constexpr uint32_t idesc_s = make_idesc_fmt(128, 128, false, false, FMT);   // S, dP: both operands K-major
   constexpr uint32_t idesc_g = make_idesc_fmt(128, D, false, true, FMT);      // gradients: B MN-major
-  const int quarter = warp & 3, half = (warp - 2) >> 2;
+  const int quarter = warp & 3, half = (warp - 4) >> 2;
   const int r = 32 * quarter + lane;                                          // row of the tile == TMEM lane
   const uint32_t lane_addr = static_cast<uint32_t>(32 * quarter) << 16;
 
@@ -333,17 +360,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         for (int t = 0; t < n && ok; ++t) {
           const int so = t & 1;
-          // P(t) written over S(t), the next Q and dO loaded (warp 10 arrives for them): dV, then the next S
+          // P(t) written over S(t), the next Q and dO loaded (warp 2 arrives for them): dV, then the next S
           // over P(t) (MMAs run in the order they are issued)
           if (!ready(kP, t & 1)) { ok = false; break; }
-          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, t > 0);
+          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, t > 0, 64, 0);
+          if (!ready(kP + 1, t & 1)) { ok = false; break; }
+          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, true, 64, 1);
           umma_commit(bars + kEmpty + 5 + so);
           if (t + 1 < n) {
             mma_ss<NKB>(t_s, sK, sQ + ((t + 1) % 3) * TILE, idesc_s);
             umma_commit(bars + kS);
           }
           if (!ready(kDs, t & 1)) { ok = false; break; }
-          mma_ts(t_dk, t_dp, sQ + (t % 3) * TILE, idesc_g, t > 0);
+          mma_ts(t_dk, t_dp, sQ + (t % 3) * TILE, idesc_g, t > 0, 64);
           umma_commit(bars + kEmpty + 2 + t % 3);
           if (t + 1 < n) {
             mma_ss<NKB>(t_dp, sV, sO + (so ^ 1) * TILE, idesc_s);
@@ -354,22 +383,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         else give_up(g, abort_flag, kErrTimeoutMma);
       }
       __syncwarp();
-    } else if (warp == 10) {
+    } else if (warp == 2) {
       // Waits for the loads in the issuer's place: its polls queue behind the MMAs it has issued (150 to
       // 270 cycles each, with the tensor cores idle), so it is left with two per tile.
       if (lane == 0 && n > 0) {
         bool ok = true;
         for (int t = 0; t < n && ok; ++t) {
-          if (t > 0) ok = wait_one<false>(bars + kP, (t - 1) & 1, abort_flag);
+          if (t > 0) ok = wait_one<false>(bars + kP + 1, (t - 1) & 1, abort_flag);
           if (ok && t + 1 < n)
             ok = wait_one<false>(bars + kFull + 2 + (t + 1) % 3, ((t + 1) / 3) & 1, abort_flag) &&
                  wait_one<false>(bars + kFull + 5 + ((t + 1) & 1), ((t + 1) >> 1) & 1, abort_flag);
-          if (ok) mbar_arrive(bars + kP);
+          if (ok) mbar_arrive(bars + kP + 1);
         }
         if (!ok) give_up(g, abort_flag, kErrTimeoutMma);
       }
       __syncwarp();
-    } else {
+    } else if (warp >= 4) {
       const int64_t key = static_cast<int64_t>(kt) * AN + r;
       const bool key_seen = key >= lo && key < hi;
       bool ok = true;
@@ -401,28 +430,30 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         {
           uint32_t v[64];
           tmem_ld64(t_s + lane_addr + half * 64, v);
+          // P by halves, so that dV begins while the second half's exponentials run
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            const float4 m = nl[c >> 2];
-            p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, m.x));
-            p[c + 1] = fast_exp2(fmaf(__uint_as_float(v[c + 1]), g.scale_log2, m.y));
-            p[c + 2] = fast_exp2(fmaf(__uint_as_float(v[c + 2]), g.scale_log2, m.z));
-            p[c + 3] = fast_exp2(fmaf(__uint_as_float(v[c + 3]), g.scale_log2, m.w));
+          for (int part = 0; part < 2; ++part) {
+#pragma unroll
+            for (int c = 32 * part; c < 32 * part + 32; c += 4) {
+              const float4 m = nl[c >> 2];
+              p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, m.x));
+              p[c + 1] = fast_exp2(fmaf(__uint_as_float(v[c + 1]), g.scale_log2, m.y));
+              p[c + 2] = fast_exp2(fmaf(__uint_as_float(v[c + 2]), g.scale_log2, m.z));
+              p[c + 3] = fast_exp2(fmaf(__uint_as_float(v[c + 3]), g.scale_log2, m.w));
+            }
+            if (!all_seen) {
+#pragma unroll
+              for (int c = 32 * part; c < 32 * part + 32; ++c) p[c] = c >= c_lo ? p[c] : 0.0f;
+            }
+            uint32_t w[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) w[c] = pack16<FMT>(p[32 * part + 2 * c], p[32 * part + 2 * c + 1]);
+            tmem_st16(t_s + lane_addr + half * 64 + 16 * part, w);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kP + part);
           }
         }
-        if (!all_seen) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) p[c] = c >= c_lo ? p[c] : 0.0f;
-        }
-        {
-          uint32_t w[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
-          tmem_st32(t_s + lane_addr + half * 64, w);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kP);
         if (!warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         uint32_t w[32];
@@ -528,8 +559,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         armed.wait_all(bars);
       }
       __syncwarp();
-    } else if (warp == 1 || warp == 10) {
-      // Two issuers: warp 1 dQ(t), S(t+2) into the buffer of dS(t); warp 10 dP(t+1) once dP(t) is read.
+    } else if (warp == 1 || warp == 2) {
+      // Two issuers: warp 1 dQ(t), S(t+2) into the buffer of dS(t); warp 2 dP(t+1) once dP(t) is read.
       if (n > 0 && elect_one()) {
         auto ready = [&](int bar, uint32_t parity) -> bool {
           if (!wait_one(bars + bar, parity, abort_flag)) return false;
@@ -551,14 +582,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           for (int t = 0; t < n && ok; ++t) {
             if (t + 2 < n && !ready(kFull + 2 + (t + 2) % 3, ((t + 2) / 3) & 1)) { ok = false; break; }
             if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
-            mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0);
+            mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0, 64);
             umma_commit(bars + kEmpty + 2 + t % 3);
             if (t + 2 < n) issue_s(t + 2);
           }
         } else {
           ok = ok && ready(kFull + 1, 0);
           for (int t = 0; t < n && ok; ++t) {
-            if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1) || (t > 0 && !ready(kDs + ((t - 1) & 1), ((t - 1) >> 1) & 1))) { ok = false; break; }
+            if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1) || (t > 0 && !ready(kP, (t - 1) & 1))) { ok = false; break; }
             mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
             umma_commit(bars + kDp);
             umma_commit(bars + kEmpty + 5 + (t & 1));
@@ -568,7 +599,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         else give_up(g, abort_flag, kErrTimeoutMma);
       }
       __syncwarp();
-    } else {
+    } else if (warp >= 4) {
       const int64_t row = static_cast<int64_t>(qt) * AM + r;
       const bool row_in = row < g.sq;
       const float* st = g.stats + (bh * g.nqt + qt) * 256;
@@ -582,6 +613,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (lane == 0) waited = mbar_wait(bars + kStall, 0, kStallLimitCycles);
         ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
       }
+      uint32_t s_here = 0;   // a look at the next S
       for (int t = 0; t < n && ok; ++t) {
         const int64_t key0 = static_cast<int64_t>(first + t) * AN;
         const int64_t a0 = lo - key0 - 64 * half, a1 = end - key0 - 64 * half;
@@ -589,25 +621,32 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int c_hi = a1 < 0 ? 0 : (a1 > 64 ? 64 : static_cast<int>(a1));
         const bool all_seen = __all_sync(0xffffffffu, c_lo == 0 && c_hi == 64);
         const uint32_t my_s = t_s + 128 * (t & 1) + lane_addr + half * 64;
-        if (!warp_wait(bars + kS + (t & 1), (t >> 1) & 1, abort_flag)) { ok = false; break; }
+        if (!looked_or_wait(s_here, bars + kS + (t & 1), (t >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         float p[64];
+        uint32_t dp_here;
         {
           uint32_t v[64];
           tmem_ld64(my_s, v);
 #pragma unroll
-          for (int c = 0; c < 64; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
+          for (int c = 0; c < 32; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
+          dp_here = look(bars + kDp, t & 1);
+#pragma unroll
+          for (int c = 32; c < 64; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
         }
-        if (!warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
+        if (!looked_or_wait(dp_here, bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
+        {
+          uint32_t v[64];
+          tmem_ld64(t_dp + lane_addr + half * 64, v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kP);   // dP(t) read: the next one may be formed
+          s_here = look(bars + kS + ((t + 1) & 1), ((t + 1) >> 1) & 1);
 #pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
-          uint32_t v[32];
-          tmem_ld32(t_dp + lane_addr + half * 64 + ch * 32, v);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) p[ch * 32 + c] *= __uint_as_float(v[c]) - delta;
+          for (int c = 0; c < 64; ++c) p[c] *= __uint_as_float(v[c]) - delta;
         }
-        if (!all_seen) {
+        if (!all_seen) {   // a masked pair's dP may be anything (V of a key outside the range)
 #pragma unroll
           for (int c = 0; c < 64; ++c) p[c] = c >= c_lo && c < c_hi ? p[c] : 0.0f;
         }
@@ -656,7 +695,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   __syncthreads();
   if (*reinterpret_cast<volatile int*>(abort_flag)) {   // every role has ended: the same answer in all threads
     // the MMAs that an aborted CTA issued end before its TMEM is released (bounded)
-    if ((warp == 1 || warp == 10) && elect_one()) {
+    if ((warp == 1 || warp == 2) && elect_one()) {
       uint64_t* drained = bars + kDrain + (warp == 1 ? 0 : 1);
       umma_commit(drained);
       mbar_wait(drained, 0);
