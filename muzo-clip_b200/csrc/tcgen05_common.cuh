@@ -367,8 +367,13 @@ __device__ __forceinline__ void pair_abort(int* flag) {
     asm volatile("st.release.cluster.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(a, r)), "r"(1) : "memory");
 }
 
-// The driver's tensor-map encoder, looked up once (thread-safe static initialisation).
+// The driver's tensor-map encoder, looked up once (thread-safe static initialisation). Encoding needs
+// a context on the calling thread, and a thread's first runtime call that would bind one may be the
+// kernel launch behind it (autograd's backward thread, with all its allocations cached): the current
+// device's context is bound here.
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;

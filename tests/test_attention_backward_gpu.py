@@ -339,6 +339,31 @@ def test_another_stream_and_two_at_once(device):
         assert all(torch.equal(a, c) for a, c in zip(g, w))
 
 
+def test_a_thread_without_a_context(device):
+    """Forward and backward as the first CUDA work of a new thread, whose allocations all come from
+    the cache: nothing before the kernels has bound the device's context to it."""
+    import threading
+
+    from muzo_clip_b200 import attention_max, attention_max_backward
+    from muzo_clip_b200.attention import _forward
+
+    q, k, v, dout = _states(device, BF16, 1, 4, 2, 200, 200, 64, seed=40)
+
+    def run():
+        out, lse, _, _ = _forward(q, k, v, 0.125, True, None, None, False, True)
+        return [attention_max(q, k, v, 0.125, True)[0], *attention_max_backward(dout, q, k, v, out, lse, 0.125, True)]
+
+    want = run()
+    run()          # leaves blocks of every size in the cache
+    got = []
+    for _ in range(3):
+        thread = threading.Thread(target=lambda: got.append(run()))
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 3 and all(torch.equal(a, c) for g in got for a, c in zip(g, want))
+
+
 def test_captured_and_replayed(device):
     """Two graphs of forward and backward (torch.autograd.grad, one key head: divided work with a
     workspace), replayed in turn on new inputs."""
