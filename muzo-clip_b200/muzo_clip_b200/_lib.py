@@ -144,6 +144,16 @@ class MuzoError(RuntimeError):
     """A native entry point returned a non-zero status."""
 
 
+try:
+    from . import _native as native  # the gradient operators' calls from torch tensors
+except ImportError as e:
+    raise ImportError(
+        f"muzo_clip_b200: the native module _native failed to load ({e}); build it with "
+        "`python muzo-clip_b200/build.py` against the installed torch"
+    ) from e
+native.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTED}, MuzoError)
+
+
 # Kernels each compute entry point enqueues (for launch accounting by benchmarks).
 KERNELS_PER_CALL = {
     "muzo_fill_noise": 1, "muzo_perturb_segments": 1, "muzo_perturb_segments_keep_noise": 1,
@@ -195,26 +205,6 @@ def dist_code(distribution: str) -> int:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-class _Here:
-    """The current device already is the one asked for."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """Context in which launches go to ``device``: the library launches on the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
 
 
 _DEVICE_PROPS: dict[int, tuple[int, int]] = {}
