@@ -22,8 +22,6 @@ constexpr int kThreads = 256;
 // CTAs of a launch: what is resident at once (at most 42 and 51 registers a thread)
 constexpr int kNormPerSm = 6, kScalePerSm = 5;
 constexpr int kMaxCtas = 148 * kNormPerSm;  // and partial sums of a launch
-constexpr int kVec = 8;                     // elements per thread and load
-constexpr int kSweep = kThreads * kVec;     // elements a CTA touches at once
 constexpr int kSmallTable = 140;            // tensors in a launch whose parameters fit 4 KB
 constexpr int kLargeTable = 1150;           // ... 32 KB
 
@@ -64,21 +62,59 @@ __device__ __forceinline__ float max_abs_nan(float m, float x) {
   return d;
 }
 
-// Sum of squares of 8 values. The squares are added in fp32 where that is safe; a sum outside
+// V consecutive elements, loaded and stored as one access of 8 or 16 bytes each; LAST: nothing reads
+// them again (the norm's reads stay in L2 for the scaling).
+template <int DTYPE, bool LAST = true, int V>
+__device__ __forceinline__ void load_vec(const char* p, float (&v)[V]) {
+  if constexpr (DTYPE == MUZO_F32) {
+    static_assert(V == 4, "16 bytes of fp32");
+    const float4 a = LAST ? __ldcs(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+    uint32_t w[V / 2];
+    if constexpr (V == 8) {
+      const uint4 u = LAST ? __ldcs(reinterpret_cast<const uint4*>(p)) : *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint2 u = LAST ? __ldcs(reinterpret_cast<const uint2*>(p)) : *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x; w[1] = u.y;
+    }
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q) {
+      v[2 * q] = DTYPE == MUZO_BF16 ? bf16_lo(w[q]) : half_lo(w[q]);
+      v[2 * q + 1] = DTYPE == MUZO_BF16 ? bf16_hi(w[q]) : half_hi(w[q]);
+    }
+  }
+}
+template <int DTYPE, int V>
+__device__ __forceinline__ void store_vec(char* p, const float (&v)[V]) {
+  if constexpr (DTYPE == MUZO_F32) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  } else {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q)
+      w[q] = DTYPE == MUZO_BF16 ? pack_bf16(v[2 * q], v[2 * q + 1]) : pack_half(v[2 * q], v[2 * q + 1]);
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
+// Sum of squares of a few values. The squares are added in fp32 where that is safe; a sum outside
 // [1e-30, 1e37], or not finite, is formed again in fp64 (squares of fp32 values reach 1e77, and
 // those of small ones vanish).
-__device__ __forceinline__ double sum8(const float (&v)[8]) {
+template <int V>
+__device__ __forceinline__ double sum_squares(const float (&v)[V]) {
   float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s = fmaf(v[k], v[k], s);
+  for (int k = 0; k < V; ++k) s = fmaf(v[k], v[k], s);
   if (s >= 1e-30f && s <= 1e37f) return s;
   uint32_t any = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) any |= __float_as_uint(v[k]);
+  for (int k = 0; k < V; ++k) any |= __float_as_uint(v[k]);
   if ((any & 0x7fffffffu) == 0) return 0.0;
   double d = 0.0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) d = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), d);
+  for (int k = 0; k < V; ++k) d = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), d);
   return d;
 }
 
@@ -87,12 +123,13 @@ template <bool INF>
 struct Total {
   double sum = 0.0;
   float top = 0.0f;
-  __device__ __forceinline__ void add8(const float (&v)[8]) {
+  template <int V>
+  __device__ __forceinline__ void add_vec(const float (&v)[V]) {
     if (INF) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = max_abs_nan(top, v[k]);
+      for (int k = 0; k < V; ++k) top = max_abs_nan(top, v[k]);
     } else {
-      sum += sum8(v);
+      sum += sum_squares(v);
     }
   }
   __device__ __forceinline__ void add(float v) {
@@ -132,25 +169,25 @@ __device__ __forceinline__ int elem_size(int dtype) { return dtype == MUZO_F32 ?
 
 template <bool INF, int DTYPE>
 __device__ __forceinline__ void norm_chunk(const char* base, int64_t n, Total<INF>& total) {
-  constexpr int size = DTYPE == MUZO_F32 ? 4 : 2;
+  constexpr int size = DTYPE == MUZO_F32 ? 4 : 2, V = 16 / size, sweep = kThreads * V;
   const int64_t head = head_elements(reinterpret_cast<uint64_t>(base), size, n);
   if (threadIdx.x < head) total.add(load_elem(base, threadIdx.x, DTYPE));
   const char* body = base + head * size;
   const int64_t m = n - head;
-  int64_t i = threadIdx.x * kVec;
-  for (; i + 3 * kSweep + kVec <= m; i += 4 * kSweep) {   // four loads in flight per thread
-    float v[4][8];
+  int64_t i = threadIdx.x * V;
+  for (; i + 3 * sweep + V <= m; i += 4 * sweep) {   // four loads in flight per thread
+    float v[4][V];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load8(body, i + u * kSweep, DTYPE, v[u]);
+    for (int u = 0; u < 4; ++u) load_vec<DTYPE, false>(body + (i + u * sweep) * size, v[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) total.add8(v[u]);
+    for (int u = 0; u < 4; ++u) total.add_vec(v[u]);
   }
-  for (; i + kVec <= m; i += kSweep) {
-    float v[8];
-    load8(body, i, DTYPE, v);
-    total.add8(v);
+  for (; i + V <= m; i += sweep) {
+    float v[V];
+    load_vec<DTYPE, false>(body + i * size, v);
+    total.add_vec(v);
   }
-  for (; i < m; ++i) total.add(load_elem(body, i, DTYPE));   // the one thread whose 8 straddle the end
+  for (; i < m; ++i) total.add(load_elem(body, i, DTYPE));   // the one thread whose V straddle the end
 }
 
 template <int N, bool INF>
@@ -194,12 +231,15 @@ __global__ void __launch_bounds__(kThreads) grad_norm_finish_kernel(const double
 }
 
 // out = dst dtype(factor * g) of one chunk; vector path where source and destination can both be
-// read and written in 16-byte pieces from the same element on.
+// accessed in whole vectors from the same element on. A vector has 16 bytes of the wider type, so that
+// a warp's stores are contiguous (with 8 elements to fp32, each store instruction wrote half of every
+// 32-byte sector it touched: 4.8 TB/s over six Llama-3-8B-shaped layers).
 template <int SRC, int DST>
 __device__ __forceinline__ void scale_chunk(const char* src, char* dst, int64_t n, float f) {
   constexpr int ss = SRC == MUZO_F32 ? 4 : 2, ds = DST == MUZO_F32 ? 4 : 2;
-  const int64_t head = head_elements(reinterpret_cast<uint64_t>(src), ss, n);
-  if (((reinterpret_cast<uint64_t>(dst) + head * ds) & 15u) != 0) {
+  constexpr int V = DST == MUZO_F32 ? 4 : 8, U = 16 / ss * 4 / V, sweep = kThreads * V;   // U loads: 64 bytes
+  int64_t head = head_elements(reinterpret_cast<uint64_t>(dst), ds, n);
+  if (((reinterpret_cast<uint64_t>(src) + head * ss) & (V * ss - 1)) != 0) {
     for (int64_t i = threadIdx.x; i < n; i += kThreads) store_elem(dst, i, DST, load_elem(src, i, SRC) * f);
     return;
   }
@@ -207,24 +247,24 @@ __device__ __forceinline__ void scale_chunk(const char* src, char* dst, int64_t 
   src += head * ss;
   dst += head * ds;
   const int64_t m = n - head;
-  int64_t i = threadIdx.x * kVec;
-  for (; i + 3 * kSweep + kVec <= m; i += 4 * kSweep) {
-    float v[4][8];
+  int64_t i = threadIdx.x * V;
+  for (; i + (U - 1) * sweep + V <= m; i += U * sweep) {
+    float v[U][V];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load8(src, i + u * kSweep, SRC, v[u]);
+    for (int u = 0; u < U; ++u) load_vec<SRC>(src + (i + u * sweep) * ss, v[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[u][k] *= f;
-      store8(dst, i + u * kSweep, DST, v[u]);
+      for (int k = 0; k < V; ++k) v[u][k] *= f;
+      store_vec<DST>(dst + (i + u * sweep) * ds, v[u]);
     }
   }
-  for (; i + kVec <= m; i += kSweep) {
-    float v[8];
-    load8(src, i, SRC, v);
+  for (; i + V <= m; i += sweep) {
+    float v[V];
+    load_vec<SRC>(src + i * ss, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= f;
-    store8(dst, i, DST, v);
+    for (int k = 0; k < V; ++k) v[k] *= f;
+    store_vec<DST>(dst + i * ds, v);
   }
   for (; i < m; ++i) store_elem(dst, i, DST, load_elem(src, i, SRC) * f);
 }
