@@ -164,18 +164,44 @@ __device__ __forceinline__ void query_tile_keys(const BwdArgs& g, int b, int qt,
   count = end > lo ? static_cast<int>((end + AN - 1) / AN) - first : 0;
 }
 
-// 32 accumulator columns of this thread's row, times f, as 16-bit values at `dst` (columns col0.. of hd).
-template <int FMT>
-__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&v)[32], float f, int col0, int hd) {
+// Rows of an accumulator to global memory, one warp: this thread's row of 128 bytes (`w`, 8 pieces of 16)
+// goes through 4 KB of shared memory, so that 8 lanes write one row's 128 bytes (a thread that wrote its
+// own row touched 32 rows with every instruction: 8000 cycles for a key CTA's 64 KB). `dst` is the
+// warp's first row at the first of these columns, `pitch` the bytes between rows; `rows` rows and
+// `pieces` pieces of each exist.
+__device__ __forceinline__ void store_rows(uint8_t* stage, const uint4 (&w)[8], uint8_t* dst, int64_t pitch, int64_t rows,
+                                           int pieces) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();   // the last call's reads are done
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (col0 + 8 * q >= hd) break;
-    uint32_t w[4];
+  for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = w[c];
+  __syncwarp();
+  const int c = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * i + (lane >> 3);
+    const uint4 x = *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+    if (row < rows && c < pieces) *reinterpret_cast<uint4*>(dst + row * pitch + 16 * c) = x;
+  }
+}
+
+// 64 accumulator columns times f as 16-bit values, 32 as fp32.
+template <int FMT>
+__device__ __forceinline__ void pack_row(const uint32_t (&v)[64], float f, uint4 (&w)[8]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      w[e] = pack16<FMT>(__uint_as_float(v[8 * q + 2 * e]) * f, __uint_as_float(v[8 * q + 2 * e + 1]) * f);
-    *reinterpret_cast<uint4*>(dst + col0 + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+      x[e] = pack16<FMT>(__uint_as_float(v[8 * c + 2 * e]) * f, __uint_as_float(v[8 * c + 2 * e + 1]) * f);
+    w[c] = make_uint4(x[0], x[1], x[2], x[3]);
   }
+}
+__device__ __forceinline__ void scale_row(const uint32_t (&v)[32], float f, uint4 (&w)[8]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    w[c] = make_uint4(__float_as_uint(__uint_as_float(v[4 * c]) * f), __float_as_uint(__uint_as_float(v[4 * c + 1]) * f),
+                      __float_as_uint(__uint_as_float(v[4 * c + 2]) * f), __float_as_uint(__uint_as_float(v[4 * c + 3]) * f));
 }
 
 // Barriers of both kinds of CTA.
@@ -489,29 +515,40 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (!ok) {
         if (lane == 0) give_up(g, abort_flag, kErrTimeoutEpilogue);
       } else if (g.parts == 1 || n > 0) {
-        // the first four warps write dV, the others c dK: one key per thread
+        // the first four warps write dV, the others c dK, 32 keys each; the operand stages are free now
         const uint32_t acc = (half == 0 ? t_dv : t_dk) + lane_addr;
         const float f = half == 0 ? 1.0f : g.scale;
-        uint16_t* out = half == 0 ? g.dv : g.dk;
-        const int64_t at = half == 0 ? b * g.dv_sb + kvh * g.dv_sh + key * g.dv_ss : b * g.dk_sb + kvh * g.dk_sh + key * g.dk_ss;
-        float* sum = g.partial + (((static_cast<int64_t>(part) * g.batch * g.hkv + bh) * g.nkt * AN + key) * 2 + half) * D;
+        uint8_t* stage = smem + 2 * TILE + (warp - 4) * 4096;
+        const int64_t key0 = static_cast<int64_t>(kt) * AN + 32 * quarter;
+        if (g.parts > 1) {
+          uint8_t* sum = reinterpret_cast<uint8_t*>(
+              g.partial + (((static_cast<int64_t>(part) * g.batch * g.hkv + bh) * g.nkt * AN + key0) * 2 + half) * D);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          if (n > 0) {
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            uint4 w[8];
             tmem_ld32(acc + c * 32, v);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0u;
+            scale_row(v, f, w);
+            store_rows(stage, w, sum + c * 128, 2 * D * 4, 32, 8);
           }
-          if (g.parts > 1) {
+        } else {
+          uint16_t* out = half == 0 ? g.dv : g.dk;
+          if (out != nullptr) {
+            const int64_t ss = half == 0 ? g.dv_ss : g.dk_ss;
+            out += half == 0 ? b * g.dv_sb + kvh * g.dv_sh + key0 * ss : b * g.dk_sb + kvh * g.dk_sh + key0 * ss;
+#pragma unroll 1
+            for (int c = 0; c < D / 64; ++c) {
+              uint4 w[8];
+              if (n > 0) {
+                uint32_t v[64];
+                tmem_ld64(acc + c * 64, v);
+                pack_row<FMT>(v, f, w);
+              } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(sum + c * 32 + e) =
-                  make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f,
-                              __uint_as_float(v[e + 3]) * f);
-          } else if (out != nullptr && key < g.sk) {
-            store_row32<FMT>(out + at, v, f, c * 32, g.hd);
+                for (int e = 0; e < 8; ++e) w[e] = make_uint4(0u, 0u, 0u, 0u);
+              }
+              store_rows(stage, w, reinterpret_cast<uint8_t*>(out + c * 64), ss * 2, g.sk - key0, (g.hd - c * 64) / 8);
+            }
           }
         }
       }
@@ -675,17 +712,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (!ok) {
         if (lane == 0) give_up(g, abort_flag, kErrTimeoutEpilogue);
       } else {
-        uint16_t* out = g.dq + b * g.dq_sb + h * g.dq_sh + row * g.dq_ss;
-#pragma unroll 1
-        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
-          uint32_t v[32];
+        // 32 rows and, of 128 columns, one half per warp; of 64, the first four warps' all
+        if (D == 128 || half == 0) {
+          const int col0 = D == 128 ? 64 * half : 0;
+          const int64_t row0 = static_cast<int64_t>(qt) * AM + 32 * quarter;
+          uint4 w[8];
           if (n > 0) {
-            tmem_ld32(t_dq + lane_addr + c * 32, v);
+            uint32_t v[64];
+            tmem_ld64(t_dq + lane_addr + col0, v);
+            pack_row<FMT>(v, g.scale, w);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0u;
+            for (int e = 0; e < 8; ++e) w[e] = make_uint4(0u, 0u, 0u, 0u);
           }
-          if (row_in) store_row32<FMT>(out, v, g.scale, c * 32, g.hd);
+          store_rows(smem + 2 * TILE + (warp - 4) * 4096, w,
+                     reinterpret_cast<uint8_t*>(g.dq + b * g.dq_sb + h * g.dq_sh + row0 * g.dq_ss + col0), g.dq_ss * 2,
+                     g.sq - row0, (g.hd - col0) / 8);
         }
       }
     }
