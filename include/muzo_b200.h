@@ -365,7 +365,7 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
  * muzo_attention_backward_workspace(...) bytes (negative: a shape this call refuses), 16-byte
  * aligned, that no other call uses until this one has finished. d_status as in muzo_attention_max. */
 int64_t muzo_attention_backward_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q,
-                                          int64_t seq_k, int64_t head_dim);
+                                          int64_t seq_k, int64_t head_dim, int causal);
 int muzo_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* dout,
                             const float* lse, void* dq, void* dk, void* dv, int dtype, int64_t batch, int64_t hq,
                             int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim, const int64_t* strides,

@@ -835,17 +835,29 @@ int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
   return launch_status();
 }
 
-// Parts that the (head, query tile) pairs of a key tile are divided into: enough CTAs to fill the
-// GPU where few key tiles exist, none with less than four pairs.
-int64_t key_parts(int64_t batch, int64_t hkv, int64_t group, int64_t nqt, int64_t nkt) {
-  const int64_t items = batch * hkv * nkt;
+// Parts that the (head, query tile) pairs of a key tile are divided into, of four pairs at least: the
+// fewest with which the longest key CTA does not outlast the average SM by more than 15 % (a division
+// costs the sums' way through memory and a launch). In units of one pair of a key CTA, a pair of a query
+// CTA takes 0.85 and a CTA's start and end 2.5 (2800, 2400 and 7000 cycles); causal CTAs start longest
+// first, and the short query CTAs fill what is left. Measured, us for 1 / 2 / 3 / 4 / 8 parts: 32 query
+// and 8 key heads, 2048 tokens 125 / 146 / 157 / 167 / 198; 8 and 1 heads, 2048 tokens 226 / 122 / 88 /
+// 71 / 45; 8 and 1 heads, 16384 tokens 1783 / 1476 / 1583 / 1569 / 1491.
+int64_t key_parts(int64_t batch, int64_t hkv, int64_t group, int64_t nqt, int64_t nkt, bool causal, bool queries) {
+  const double sms = 148.0, query_step = 0.85, cta = 2.5;
   const int64_t pairs = group * nqt;
-  const int64_t sms = 148;
-  if (items <= 0) return 1;
-  int64_t parts = (2 * sms + items - 1) / items;
-  if (parts > pairs / 4) parts = pairs / 4;
-  if (parts > 32) parts = 32;
-  return parts < 1 ? 1 : parts;
+  if (batch <= 0 || nkt <= 0 || pairs <= 1) return 1;
+  double tiles = static_cast<double>(nqt) * static_cast<double>(nkt);   // visible tile pairs of a head
+  if (causal) {
+    const double m = static_cast<double>(nqt < nkt ? nqt : nkt);
+    tiles = nqt <= nkt ? tiles - m * (m - 1) / 2 : m * (m + 1) / 2;
+  }
+  const double heads = static_cast<double>(batch) * static_cast<double>(hkv * group);
+  const double items = static_cast<double>(batch) * static_cast<double>(hkv) * static_cast<double>(nkt);
+  const double steps = heads * tiles * (queries ? 1.0 + query_step : 1.0) + (queries ? heads * nqt * cta : 0.0);
+  const int64_t most = pairs / 4 < 32 ? pairs / 4 : 32;
+  for (int64_t parts = 1; parts < most; ++parts)
+    if (static_cast<double>((pairs + parts - 1) / parts) + cta <= 1.15 * (steps + items * parts * cta) / sms) return parts;
+  return most > 1 ? most : 1;
 }
 
 int64_t stats_bytes(int64_t batch, int64_t hq, int64_t nqt) { return batch * hq * nqt * 1024; }
@@ -866,10 +878,11 @@ using namespace muzo;
 extern "C" {
 
 int64_t muzo_attention_backward_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k,
-                                          int64_t head_dim) {
+                                          int64_t head_dim, int causal) {
   if (bwd_shape(dtype, batch, hq, hkv, seq_q, seq_k, head_dim) != MUZO_OK) return -1;
   const int64_t nqt = (seq_q + AM - 1) / AM, nkt = (seq_k + AN - 1) / AN;
-  const int64_t parts = key_parts(batch, hkv, hq / hkv, nqt, nkt);
+  // without dQ the key tiles are divided into at least as many parts as with it
+  const int64_t parts = key_parts(batch, hkv, hq / hkv, nqt, nkt, causal != 0, false);
   const int64_t sums = parts > 1 ? parts * batch * hkv * nkt * AN * 2 * (head_dim <= 64 ? 64 : 128) * 4 : 0;
   return stats_bytes(batch, hq, nqt) + sums + 16;
 }
@@ -893,7 +906,7 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
   for (const void* p : bases)
     if (!aligned16p(p)) return MUZO_ERR_ALIGN;
   if (!none && !aligned16p(d_workspace)) return MUZO_ERR_ALIGN;
-  if (!none && workspace_bytes < muzo_attention_backward_workspace(dtype, batch, hq, hkv, seq_q, seq_k, head_dim))
+  if (!none && workspace_bytes < muzo_attention_backward_workspace(dtype, batch, hq, hkv, seq_q, seq_k, head_dim, causal))
     return MUZO_ERR_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   BwdArgs g = {};
@@ -902,7 +915,7 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
   g.group = static_cast<int>(hq / hkv); g.hd = static_cast<int>(head_dim); g.causal = causal ? 1 : 0;
   g.nqt = static_cast<int>((seq_q + AM - 1) / AM);
   g.nkt = static_cast<int>((seq_k + AN - 1) / AN);
-  g.parts = static_cast<int>(key_parts(batch, hkv, g.group, g.nqt, g.nkt));
+  g.parts = static_cast<int>(key_parts(batch, hkv, g.group, g.nqt, g.nkt, causal != 0, dq != nullptr));
   g.scale = scale; g.scale_log2 = scale * kLog2e;
   g.key_lo = d_key_lo; g.key_hi = d_key_hi;
   g.dq = static_cast<uint16_t*>(dq); g.dk = static_cast<uint16_t*>(dk); g.dv = static_cast<uint16_t*>(dv);

@@ -215,7 +215,7 @@ std::array<Tensor, 3> attention_backward(const Tensor& grad_out, const Tensor& q
                                ds[0], ds[2], ds[1], gs[0][0], gs[0][1], gs[0][2], gs[1][0], gs[1][1], gs[1][2],
                                gs[2][0], gs[2][1], gs[2][2]};
   const int code = dtype_code(q);
-  const int64_t size = lib.attention_workspace(code, b, hq, hkv, sq, sk, d);
+  const int64_t size = lib.attention_workspace(code, b, hq, hkv, sq, sk, d, causal ? 1 : 0);
   if (size < 0) throw Failure("muzo_attention_backward: shape not supported");
   const Tensor workspace = at::empty({size}, q.options().dtype(at::kByte));
   check(lib.attention_backward(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), lse.const_data_ptr<float>(), out_ptr(grads[0]),

@@ -118,7 +118,7 @@ _SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _i32] + [_i64] * 6 + [_i64] * 12 + [_i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp],
         _i32,
     ),
-    "muzo_attention_backward_workspace": ([_i32] + [_i64] * 6, _i64),
+    "muzo_attention_backward_workspace": ([_i32] + [_i64] * 6 + [_i32], _i64),
     "muzo_attention_backward": (
         [_vp] * 9 + [_i32] + [_i64] * 6 + [_vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp, _vp],
         _i32,

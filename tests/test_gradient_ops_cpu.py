@@ -55,12 +55,15 @@ def test_backward_workspace_sizes():
     from muzo_clip_b200 import _lib
 
     size = _lib.lib.muzo_attention_backward_workspace
-    assert size(1, 1, 4, 3, 8, 8, 64) < 0 and size(0, 1, 4, 2, 8, 8, 64) < 0 and size(1, 1, 4, 2, 8, 8, 72 + 64) < 0
+    assert size(1, 1, 4, 3, 8, 8, 64, 1) < 0 and size(0, 1, 4, 2, 8, 8, 64, 1) < 0 and size(1, 1, 4, 2, 8, 8, 72 + 64, 0) < 0
     # two fp32 values for each query row, padded to tiles of 128
     for b, hq, sq in ((1, 4, 8), (3, 32, 2048), (2, 6, 129)):
-        assert size(1, b, hq, 2, sq, sq, 128) >= 8 * b * hq * (-(-sq // 128) * 128)
+        for causal in (0, 1):
+            assert size(1, b, hq, 2, sq, sq, 128, causal) >= 8 * b * hq * (-(-sq // 128) * 128)
+    # one key head and many queries: sums of dK and dV for each part of the work
+    assert size(1, 1, 8, 1, 2048, 2048, 128, 1) >= 8 * 8 * 2048 + 2 * 2048 * 2 * 128 * 4
     # beyond 32 bits
-    assert size(1, 64, 128, 128, 1 << 20, 1 << 20, 128) > 1 << 32
+    assert size(1, 64, 128, 128, 1 << 20, 1 << 20, 128, 1) > 1 << 32
 
 
 def test_python_refuses_cpu_tensors():
