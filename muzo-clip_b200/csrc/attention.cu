@@ -36,8 +36,9 @@ using namespace tc;
 using namespace attn;
 
 constexpr int AMB = 2 * AM;      // query rows per CTA: two query tiles share each K / V tile
-constexpr int A_THREADS = 352;   // warp 0 TMA of Q and K, warp 1 MMA, warps 2..9 softmax (two streams
-                                 // of four warps, one warp per TMEM lane quarter), warp 10 TMA of V
+constexpr int A_THREADS = 384;   // warp 0 TMA of Q and K, warps 1 and 11 MMA of streams 0 and 1, warps 2..9
+                                 // softmax (two streams of four warps, one warp per TMEM lane quarter),
+                                 // warp 10 TMA of V
 constexpr int K_STAGES = 1;      // K ring depth (tile j uses K stage j % K_STAGES)
 constexpr int BOX_BYTES = 64 * ABK * 2;      // one 64 x 64 box of the MN-major V operand (8 KB)
 constexpr uint32_t TMEM_COLS = 512;          // S of each stream at 0 and 128, O of each stream from 256
@@ -147,8 +148,9 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint64_t* s_full = v_empty + VS;          // [stream]: S of the stream's next tile computed
   uint64_t* p_full = s_full + 2;            // [stream]: P written (and S read) by the stream's 4 warps
   uint64_t* o_done = p_full + 2;            // [stream]: P V of the stream's last tile done
-  uint64_t* drain = o_done + 2;
-  uint64_t* stall_bar = drain + 1;          // nothing arrives here: a stall request waits on it
+  uint64_t* s_free = o_done + 2;            // [stream]: S in registers, its buffer may take the next S
+  uint64_t* drain = s_free + 2;             // [stream]
+  uint64_t* stall_bar = drain + 2;          // nothing arrives here: a stall request waits on it
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(stall_bar + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
 
@@ -165,10 +167,12 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int s = 0; s < K_STAGES; ++s) { mbar_init(k_full + s, 1); mbar_init(k_empty + s, 1); }
-    for (int s = 0; s < VS; ++s) { mbar_init(v_full + s, 1); mbar_init(v_empty + s, 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(s_full + s, 1); mbar_init(p_full + s, 4); mbar_init(o_done + s, 1); }
-    mbar_init(drain, 1);
+    for (int s = 0; s < K_STAGES; ++s) { mbar_init(k_full + s, 1); mbar_init(k_empty + s, 2); }
+    for (int s = 0; s < VS; ++s) { mbar_init(v_full + s, 1); mbar_init(v_empty + s, 2); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full + s, 1); mbar_init(p_full + s, 4); mbar_init(o_done + s, 1); mbar_init(s_free + s, 4);
+      mbar_init(drain + s, 1);
+    }
     mbar_init(stall_bar, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -238,21 +242,31 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (armed & (1u << s2)) mbar_wait(full + s2, (armed_parity >> s2) & 1u);
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    // S_s(0) for both streams; then per tile j and stream s (in that order): once P_s(j) is
-    // written (S buffer s read), S_s(j + 1) and then O_s += P_s(j) V_j. A K stage is released after
-    // the last S that reads it, a V stage after the last P V.
-    if (lane == 0 && ntiles > 0) {
+  } else if (warp == 1 || warp == 11) {
+    // ------------------------------------------------------------------ MMA issuers, one per stream
+    // Stream s: S_s(0); then per tile j S_s(j + 1) as soon as the softmax holds S_s(j) in registers, and
+    // O_s += P_s(j) V_j once P_s(j) is written. A K or V stage is released by both issuers: by a commit
+    // behind the product that read it, or by an arrival where the stream has no such tile.
+    if (ntiles > 0 && elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_fmt(AM, AN, false, false, FMT);
       constexpr uint32_t idesc_pv = make_idesc_fmt(AM, D, false, true, FMT);
-      const int nt[2] = {n0, n1};
-      auto issue_s = [&](int s, int j) -> bool {
-        const int stage = j % K_STAGES;
-        if (!mbar_wait(k_full + stage, static_cast<uint32_t>((j / K_STAGES) & 1))) return false;
+      const int s = warp == 1 ? 0 : 1;
+      const int mine = s == 0 ? n0 : n1;
+      const uint32_t sq_ = smem_u32(sQ + s * L::Q_BYTES), sp = smem_u32(sP + s * L::P_BYTES);
+      auto ready = [&](uint64_t* bar, int phase) -> bool {
+        if (!mbar_wait(bar, static_cast<uint32_t>(phase & 1))) return false;
         if (*reinterpret_cast<volatile int*>(abort_flag)) return false;
         tc_fence_after();
-        const uint32_t sq_ = smem_u32(sQ + s * L::Q_BYTES);
+        return true;
+      };
+      auto issue_s = [&](int j) -> bool {
+        const int stage = j % K_STAGES;
+        if (!ready(k_full + stage, j / K_STAGES)) return false;
+        if (j >= mine) {
+          mbar_arrive(k_empty + stage);
+          return true;
+        }
+        if (j > 0 && !ready(s_free + s, j - 1)) return false;
         const uint32_t sk_ = smem_u32(sK + stage * L::K_BYTES);
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
@@ -261,17 +275,18 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             umma_f16(tmem_base + s * AN, make_sdesc(sq_ + kb * SUB_BYTES + k * 32, 16, 1024),
                      make_sdesc(sk_ + kb * SUB_BYTES + k * 32, 16, 1024), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
         umma_commit(s_full + s);
-        // the last stream that reads K_j (stream 1 whenever it has tile j) releases the stage
-        if (s == 1 || j >= nt[1]) umma_commit(k_empty + stage);
+        umma_commit(k_empty + stage);
         return true;
       };
-      auto issue_pv = [&](int s, int j) -> bool {
+      auto issue_pv = [&](int j) -> bool {
         const int stage = j % VS;
-        if (!mbar_wait(v_full + stage, static_cast<uint32_t>((j / VS) & 1))) return false;
-        if (*reinterpret_cast<volatile int*>(abort_flag)) return false;
-        tc_fence_after();
+        if (!ready(v_full + stage, j / VS)) return false;
+        if (j >= mine) {
+          mbar_arrive(v_empty + stage);
+          return true;
+        }
+        if (!ready(p_full + s, j)) return false;
         const uint32_t sv = smem_u32(sV + stage * L::V_BYTES);
-        const uint32_t sp = smem_u32(sP + s * L::P_BYTES);
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
@@ -279,22 +294,15 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             umma_f16(tmem_o + s * D, make_sdesc(sp + kc * SUB_BYTES + k * 32, 16, 1024),
                      make_sdesc(sv + kc * NKB * BOX_BYTES + k * (16 * 128), BOX_BYTES, 1024), idesc_pv,
                      (j > 0 || kc > 0 || k > 0) ? 1u : 0u);
-        if (s == 1 || j >= nt[1]) umma_commit(v_empty + stage);   // V_j read by both streams
+        umma_commit(v_empty + stage);
         umma_commit(o_done + s);        // P buffer of the stream free, O_s holds its tiles up to j
         return true;
       };
       bool ok = stall != kErrTimeoutMma || mbar_wait(stall_bar, 0, kStallLimitCycles);
-      ok = ok && mbar_wait(q_full, 0);
-      for (int s = 0; s < 2 && ok; ++s)
-        if (nt[s] > 0) ok = issue_s(s, 0);
+      ok = ok && ready(q_full, 0) && issue_s(0);
       for (int j = 0; j < ntiles && ok; ++j) {
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (j >= nt[s]) continue;
-          if (!mbar_wait(p_full + s, static_cast<uint32_t>(j & 1))) { ok = false; break; }
-          tc_fence_after();
-          if (j + 1 < nt[s] && !issue_s(s, j + 1)) { ok = false; break; }
-          if (!issue_pv(s, j)) { ok = false; break; }
-        }
+        if (j + 1 < ntiles) ok = issue_s(j + 1);
+        ok = ok && issue_pv(j);
       }
       if (!ok) {
         atomicCAS(g.status, kErrNone, kErrTimeoutMma);
@@ -414,6 +422,11 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       for (int ch = 0; ch < 2; ++ch) {
         uint32_t v[64];
         tmem_ld64(s_cols + ch * 64, v);
+        if (ch == 1) {   // S is read: the next one may be formed while this tile's exponentials run
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free + stream);
+        }
         uint32_t packed[32];
         if (m_run == -INFINITY) {
 #pragma unroll
@@ -530,13 +543,16 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    if (lane == 0 && *reinterpret_cast<volatile int*>(abort_flag)) {
-      // drain the MMAs an aborted CTA issued before its TMEM is released (bounded)
-      umma_commit(drain);
-      mbar_wait(drain, 0);
+  if (*reinterpret_cast<volatile int*>(abort_flag)) {   // every role has ended: the same answer in all threads
+    // the MMAs that an aborted CTA issued end before its TMEM is released (bounded)
+    if ((warp == 1 || warp == 11) && elect_one()) {
+      uint64_t* drained = drain + (warp == 1 ? 0 : 1);
+      umma_commit(drained);
+      mbar_wait(drained, 0);
     }
-    __syncwarp();
+    __syncthreads();
+  }
+  if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
                  : "memory");
