@@ -122,7 +122,7 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return d;
 }
 
-template <int FMT, int D>
+template <int FMT, int D, bool REC>
 __global__ void __launch_bounds__(A_THREADS, 1)
 attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, AttnArgs g) {
@@ -354,7 +354,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (c_hi < c_lo) c_hi = c_lo;
       }
       const bool all_visible = c_lo == 0 && c_hi == AN;
-      // pass 1: the tile's maximum and minimum over the visible logits
+      // pass 1: the tile's maximum (and, to record, minimum) over the visible logits
       float mx[4], mn[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) { mx[q] = -INFINITY; mn[q] = INFINITY; }
@@ -367,7 +367,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           for (int c = 0; c < 64; c += 2) {
             const float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
             mx[(c >> 1) & 3] = max3_nan(mx[(c >> 1) & 3], x0, x1);
-            mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], x0, x1);
+            if (REC) mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], x0, x1);
           }
         } else {
 #pragma unroll
@@ -376,13 +376,15 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool v0 = k0 >= c_lo && k0 < c_hi, v1 = k0 + 1 >= c_lo && k0 + 1 < c_hi;
             const float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
             mx[(c >> 1) & 3] = max3_nan(mx[(c >> 1) & 3], v0 ? x0 : -INFINITY, v1 ? x1 : -INFINITY);
-            mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], v0 ? x0 : INFINITY, v1 ? x1 : INFINITY);
+            if (REC) mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], v0 ? x0 : INFINITY, v1 ? x1 : INFINITY);
           }
         }
       }
       const float mt = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
-      raw_max = max3_nan(raw_max, mt, -INFINITY);
-      raw_min = min3(min3(raw_min, mn[0], mn[1]), mn[2], mn[3]);
+      if (REC) {
+        raw_max = max3_nan(raw_max, mt, -INFINITY);
+        raw_min = min3(min3(raw_min, mn[0], mn[1]), mn[2], mn[3]);
+      }
       // lazy online softmax in base 2
       const float mt2 = mt * g.scale_log2;
       float alpha = 1.0f;
@@ -522,7 +524,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           }
         }
       }
-      if (g.enc != nullptr) {
+      if (REC) {
         float m = raw_max;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = max3_nan(m, __shfl_xor_sync(0xffffffffu, m, o), -INFINITY);
@@ -559,10 +561,10 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   }
 }
 
-template <int FMT, int D>
+template <int FMT, int D, bool REC>
 int launch_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& g,
                 cudaStream_t s) {
-  auto kern = attn_fwd_max_kernel<FMT, D>;
+  auto kern = attn_fwd_max_kernel<FMT, D, REC>;
   static std::atomic<bool> configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -573,6 +575,12 @@ int launch_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap&
   }
   kern<<<static_cast<unsigned>(g.num_items), A_THREADS, AttnLayout<D>::SMEM_BYTES, s>>>(mq, mk, mv, g);
   return launch_status();
+}
+
+// With or without the maxima (whose minima, for a visible -inf, cost a third of the first pass).
+template <int FMT, int D>
+int launch_head(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& g, cudaStream_t s) {
+  return g.enc != nullptr ? launch_attn<FMT, D, true>(mq, mk, mv, g, s) : launch_attn<FMT, D, false>(mq, mk, mv, g, s);
 }
 
 __global__ void init_attn_max_kernel(int* enc, int n, int32_t* valid) {
@@ -651,9 +659,9 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
     g.hd = static_cast<int>(head_dim); g.lse = lse;
     g.enc = enc; g.valid = d_valid; g.status = d_status;
     if (dtype == MUZO_BF16)
-      st = head_dim <= 64 ? launch_attn<1, 64>(mq, mk, mv, g, s) : launch_attn<1, 128>(mq, mk, mv, g, s);
+      st = head_dim <= 64 ? launch_head<1, 64>(mq, mk, mv, g, s) : launch_head<1, 128>(mq, mk, mv, g, s);
     else
-      st = head_dim <= 64 ? launch_attn<0, 64>(mq, mk, mv, g, s) : launch_attn<0, 128>(mq, mk, mv, g, s);
+      st = head_dim <= 64 ? launch_head<0, 64>(mq, mk, mv, g, s) : launch_head<0, 128>(mq, mk, mv, g, s);
     if (st != MUZO_OK) return st;
   }
   if (enc != nullptr)
