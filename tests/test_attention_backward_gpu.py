@@ -5,7 +5,8 @@ Tolerances are the rounding steps the kernels take, summed worst case with |.| i
 factor: P and dS enter the products rounded to the input type (half a step u = eps / 2, relative,
 and half the smallest subnormal s, absolute), results are rounded once more (u), and fp32 dot
 products of n terms are off by at most n * 2^-23 of the sum of their terms' magnitudes (2^-16 for the
-128 products of a logit). With autograd, delta = dO . O uses the rounded O, u sum |dO O| off.
+128 products of a logit). With autograd, delta = dO . O uses the forward's O, which is rounded (u) and
+took P rounded (u sum P |v|).
 """
 
 from __future__ import annotations
@@ -62,7 +63,9 @@ def _exact(q, k, v, dout, scale, vis, out=None):
     # the bounds
     ga, ka, va, qa = g.abs(), kd.abs(), vd.abs(), qd.abs()
     rel_p = 2.0 ** -16 * (1 + scale * (qa @ ka.transpose(2, 3))) + 2.0 ** -22 * torch.where(lse == -math.inf, 0.0, lse.abs())[..., None]
-    err_delta = (ga * used.abs()).sum(-1, keepdim=True) * (2.0 ** -16 + (u if out is None else 0.0))
+    err_delta = (ga * used.abs()).sum(-1, keepdim=True) * 2.0 ** -16
+    if out is None:
+        err_delta = err_delta + (ga * (u * used.abs() + (u + 2.0 ** -16) * (p @ va))).sum(-1, keepdim=True)
     err_dp = 2.0 ** -16 * (ga @ va.transpose(2, 3))
     err_p = p * (rel_p + u) + s * vis
     err_ds = (ds.abs() * (u + rel_p) + p * (err_dp + err_delta)) * 1.01 + s * vis
