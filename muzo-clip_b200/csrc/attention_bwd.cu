@@ -48,7 +48,9 @@ struct BwdArgs {
   float scale, scale_log2;
   const int32_t* key_lo;
   const int32_t* key_hi;
-  const float* stats;    // [B * Hq][nqt][2][128]: -lse in log2 units (-inf: no key seen, or no such row), delta
+  const float* stats;    // [B * Hq][nqt][2][128]: -lse in log2 units (fp16: plus 10; -inf: no key seen, or no such
+                         // row), delta
+  const uint32_t* largest;  // fp16: the bits of the largest |dO_i|^2 and, of visible keys, |v_j|^2
   float* partial;        // [parts][B * Hkv][nkt * 128][2][D] sums of dV and c dK, or null when parts == 1
   uint16_t *dq, *dk, *dv;   // any may be null
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
@@ -105,6 +107,13 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const i
   }
   return true;
 }
+// s (dP - delta), s being 1 for bf16.
+template <int FMT>
+__device__ __forceinline__ float scaled_less(uint32_t dp, float delta, float s) {
+  const float x = __uint_as_float(dp) - delta;
+  return FMT == 1 ? x : x * s;
+}
+
 // A look at a barrier ahead of time, without a branch: lane 0 polls, the answer is used later by
 // `looked_or_wait`. A poll queues behind the exponentials of both warps of a scheduler (300 cycles and
 // more), which pass meanwhile.
@@ -275,6 +284,36 @@ __device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int c
   atomicExch(abort_flag, 1);
 }
 
+// Powers of two that P and dS carry on their way through 16 bits. bf16 has fp32's range and needs none.
+// In fp16 a probability below 2^-14 would lose bits, and dS, a probability times a gradient, most of them
+// (or overflow): P is taken 2^10-fold, and dS times the largest 2^k that keeps |dS| <= 2 max|dO_i| max|v_j|
+// (|delta| <= |dO_i| max|v_j|: O is a mean of the v_j) at or below 2^15. The products' results are divided
+// again in fp32.
+struct Powers {
+  float ds = 1.0f;          // factor of dP and delta: 2^(k - 10)
+  float dv = 1.0f, dqk = 1.0f;   // 2^-10 and 2^-k
+};
+template <int FMT>
+__device__ __forceinline__ Powers powers_of(const BwdArgs& g) {
+  Powers p;
+  if (FMT == 0) {
+    wait_for_statistics();
+    const float a = __uint_as_float(g.largest[0]), b = __uint_as_float(g.largest[1]);
+    const float bound = 2.0f * sqrtf(a) * sqrtf(b);
+    int k = 0;
+    if (bound > 0.0f && bound < INFINITY) {
+      int e;
+      frexpf(bound, &e);      // bound < 2^e
+      k = 15 - e;
+      k = k < -24 ? -24 : (k > 40 ? 40 : k);
+    }
+    p.ds = ldexpf(1.0f, k - 10);
+    p.dv = 1.0f / 1024.0f;
+    p.dqk = ldexpf(1.0f, -k);
+  }
+  return p;
+}
+
 template <int FMT, int D>
 __global__ void __launch_bounds__(B_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -430,6 +469,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       __syncwarp();
     } else if (warp >= 4) {
+      const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
       const int64_t key = static_cast<int64_t>(kt) * AN + r;
       const bool key_seen = key >= lo && key < hi;
       bool ok = true;
@@ -496,10 +536,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           for (int c = 0; c < 32; c += 4) {
             const float4 m = dl[(ch * 32 + c) >> 2];
             float* pp = p + ch * 32 + c;
-            pp[0] *= __uint_as_float(v[c]) - m.x;
-            pp[1] *= __uint_as_float(v[c + 1]) - m.y;
-            pp[2] *= __uint_as_float(v[c + 2]) - m.z;
-            pp[3] *= __uint_as_float(v[c + 3]) - m.w;
+            pp[0] *= scaled_less<FMT>(v[c], m.x, two.ds);
+            pp[1] *= scaled_less<FMT>(v[c + 1], m.y, two.ds);
+            pp[2] *= scaled_less<FMT>(v[c + 2], m.z, two.ds);
+            pp[3] *= scaled_less<FMT>(v[c + 3], m.w, two.ds);
           }
         }
         if (!all_seen) {   // a masked pair's dP may be anything (a key's V outside its range)
@@ -522,7 +562,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       } else if (g.parts == 1 || n > 0) {
         // the first four warps write dV, the others c dK, 32 keys each; the operand stages are free now
         const uint32_t acc = (half == 0 ? t_dv : t_dk) + lane_addr;
-        const float f = half == 0 ? 1.0f : g.scale;
+        const float f = half == 0 ? two.dv : g.scale * two.dqk;
         uint8_t* stage = smem + 2 * TILE + (warp - 4) * 4096;
         const int64_t key0 = static_cast<int64_t>(kt) * AN + 32 * quarter;
         if (g.parts > 1) {
@@ -646,6 +686,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const bool row_in = row < g.sq;
       const float* st = g.stats + (bh * g.nqt + qt) * 256;
       wait_for_statistics();
+      const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
       const float nl = n > 0 ? st[r] : 0.0f, delta = n > 0 ? st[128 + r] : 0.0f;
       int64_t end = hi;                                      // visible keys of this row: [lo, end)
       if (g.causal && row + g.shift + 1 < end) end = row + g.shift + 1;
@@ -687,7 +728,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (lane == 0) mbar_arrive(bars + kP);   // dP(t) read: the next one may be formed
           s_here = look(bars + kS + ((t + 1) & 1), ((t + 1) >> 1) & 1);
 #pragma unroll
-          for (int c = 0; c < 64; ++c) p[c] *= __uint_as_float(v[c]) - delta;
+          for (int c = 0; c < 64; ++c) p[c] *= scaled_less<FMT>(v[c], delta, two.ds);
         }
         if (!all_seen) {   // a masked pair's dP may be anything (V of a key outside the range)
 #pragma unroll
@@ -726,7 +767,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (n > 0) {
             uint32_t v[64];
             tmem_ld64(t_dq + lane_addr + col0, v);
-            pack_row<FMT>(v, g.scale, w);
+            pack_row<FMT>(v, g.scale * two.dqk, w);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = make_uint4(0u, 0u, 0u, 0u);
@@ -756,36 +797,98 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   }
 }
 
-// Per query row: -lse in log2 units (-inf for a row that sees no key, so that its probabilities are 0)
-// and delta = dO . O, in tiles of 128 rows padded with such rows. 16 lanes per row, 8 elements each.
+// The largest of the block's values (not negative, or NaN) into *word, as its bits.
+__device__ __forceinline__ void block_largest(float v, uint32_t* word) {
+  __shared__ uint32_t most;
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
+  const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
+  if ((threadIdx.x & 31) == 0) atomicMax(&most, w);
+  __syncthreads();
+  if (threadIdx.x == 0) atomicMax(word, most);   // the largest is the same in whatever order
+}
+
+// The larger of two values, NaN if either is.
+__device__ __forceinline__ float larger(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s, 16);
+  return v;
+}
+
+constexpr int kStatThreads = 512, kStatGroups = kStatThreads / 16;
+
+struct Rows16 {   // a [B][H][S][D] operand of 16-bit elements
+  const uint16_t* p;
+  int64_t sb, sh, ss;
+};
+
+// Per query row: -lse in log2 units (with the power of two that P carries; -inf for a row that sees no
+// key, so that its probabilities are 0) and delta = dO . O, in tiles of 128 rows padded with such rows: one
+// block per tile, 16 lanes per row (8 elements each), four rows per lane with their loads in flight
+// together. For fp16 also the largest |dO_i|^2 and, in the blocks behind the query tiles', the largest
+// |v_j|^2 of the keys inside their range.
 template <int FMT>
-__global__ void __launch_bounds__(256)
-attn_bwd_stats_kernel(const uint16_t* o, int64_t o_sb, int64_t o_sh, int64_t o_ss, const uint16_t* d, int64_t d_sb,
-                      int64_t d_sh, int64_t d_ss, const float* lse, float* stats, int hq, int64_t sq, int nqt, int hd,
-                      int64_t rows) {
+__global__ void __launch_bounds__(kStatThreads, 2)
+attn_bwd_stats_kernel(Rows16 o, Rows16 d, Rows16 v, const float* lse, float* stats, uint32_t* largest, int hq, int64_t sq,
+                      int nqt, int hd, unsigned query_tiles, int hkv, int64_t sk, int nkt, const int32_t* key_lo,
+                      const int32_t* key_hi) {
+  constexpr int type = FMT == 1 ? MUZO_BF16 : MUZO_F16;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;   // row of the padded [B * Hq][nqt * 128]
-  const int l = threadIdx.x & 15;
-  if (at >= rows) return;   // whole half-warps: rows is a multiple of 128
-  const int64_t bh = at / (static_cast<int64_t>(nqt) * AM), i = at % (static_cast<int64_t>(nqt) * AM);
-  float sum = 0.0f;
-  const bool in = i < sq;
-  if (in && 8 * l < hd) {
-    const int64_t b = bh / hq, h = bh % hq;
-    float x[8], y[8];
-    load8(o, b * o_sb + h * o_sh + i * o_ss + 8 * l, FMT == 1 ? MUZO_BF16 : MUZO_F16, x);
-    load8(d, b * d_sb + h * d_sh + i * d_ss + 8 * l, FMT == 1 ? MUZO_BF16 : MUZO_F16, y);
+  const int l = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const bool here = 8 * l < hd;
+  float square = 0.0f;
+  if (FMT == 0 && blockIdx.x >= query_tiles) {
+    const unsigned t = blockIdx.x - query_tiles;
+    const int bh = static_cast<int>(t / nkt), kt = static_cast<int>(t % nkt), b = bh / hkv;
+    int64_t lo, hi;
+    key_range(key_lo, key_hi, sk, b, lo, hi);
+    const uint16_t* base = v.p + b * v.sb + (bh % hkv) * v.sh + 8 * l;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
-  }
+    for (int r = 0; r < AM / kStatGroups; ++r) {
+      const int64_t j = static_cast<int64_t>(kt) * AN + kStatGroups * r + group;
+      float x[8] = {}, s = 0.0f;
+      if (here && j >= lo && j < hi) load8(base, j * v.ss, type, x);
 #pragma unroll
-  for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s, 16);
-  if (l == 0) {
-    const float v = in ? lse[bh * sq + i] : -INFINITY;
-    float* tile = stats + (at >> 7) * 256 + (at & 127);
-    tile[0] = v == -INFINITY ? -INFINITY : -v * kLog2e;
-    tile[128] = in ? sum : 0.0f;
+      for (int e = 0; e < 8; ++e) s = fmaf(x[e], x[e], s);
+      square = larger(square, sum16(s));
+    }
+    block_largest(square, largest + 1);
+    return;
   }
+  const int bh = static_cast<int>(blockIdx.x / nqt), qt = static_cast<int>(blockIdx.x % nqt), b = bh / hq, h = bh % hq;
+  const uint16_t* ob = o.p + b * o.sb + h * o.sh + 8 * l;
+  const uint16_t* db = d.p + b * d.sb + h * d.sh + 8 * l;
+  float* tile = stats + static_cast<int64_t>(blockIdx.x) * 256;
+#pragma unroll
+  for (int r = 0; r < AM / kStatGroups; ++r) {
+    const int row = kStatGroups * r + group;
+    const int64_t i = static_cast<int64_t>(qt) * AM + row;
+    const bool in = i < sq;
+    float x[8] = {}, y[8] = {}, sum = 0.0f, s = 0.0f;
+    if (here && in) {
+      load8(ob, i * o.ss, type, x);
+      load8(db, i * d.ss, type, y);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sum = fmaf(x[e], y[e], sum);
+      if (FMT == 0) s = fmaf(y[e], y[e], s);
+    }
+    sum = sum16(sum);
+    if (FMT == 0) square = larger(square, sum16(s));
+    if (l == 0) {
+      const float w = in ? lse[static_cast<int64_t>(bh) * sq + i] : -INFINITY;
+      tile[row] = w == -INFINITY ? -INFINITY : fmaf(-w, kLog2e, FMT == 0 ? 10.0f : 0.0f);   // fp16: 2^10 P
+      tile[128 + row] = in ? sum : 0.0f;
+    }
+  }
+  if (FMT == 0) block_largest(square, largest);
 }
 
 // dK, dV of every key: the sums of its tile's parts, in order.
@@ -953,7 +1056,7 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
   g.stats = stats;
   CUtensorMap mq = {}, mk = {}, mv = {}, md = {};
   if (!none) {
-    g.partial = g.parts > 1 ? stats + stats_bytes(batch, hq, g.nqt) / 4 : nullptr;
+    g.partial = g.parts > 1 ? stats + stats_bytes(batch, hq, g.nqt) / 4 + 4 : nullptr;
     st = encode_attn_map(&mq, q, dtype, head_dim, seq_q, hq, batch, strides[2], strides[1], strides[0], AM);
     if (st != MUZO_OK) return st;
     st = encode_attn_map(&mk, k, dtype, head_dim, seq_k, hkv, batch, strides[5], strides[4], strides[3], AN);
@@ -962,13 +1065,17 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
     if (st != MUZO_OK) return st;
     st = encode_attn_map(&md, dout, dtype, head_dim, seq_q, hq, batch, strides[14], strides[13], strides[12], AM);
     if (st != MUZO_OK) return st;
-    const int64_t rows = batch * hq * g.nqt * AM;
-    const int64_t blocks = rows / 16;
-    if (blocks > 0x7fffffffLL) return MUZO_ERR_UNSUPPORTED;
+    uint32_t* largest = reinterpret_cast<uint32_t*>(stats + stats_bytes(batch, hq, g.nqt) / 4);
+    g.largest = largest;
+    const int64_t query_tiles = batch * hq * g.nqt, value_tiles = dtype == MUZO_F16 ? batch * hkv * g.nkt : 0;
+    if (query_tiles + value_tiles > 0x7fffffffLL) return MUZO_ERR_UNSUPPORTED;
+    if (dtype == MUZO_F16) MUZO_CUDA_CHECK(cudaMemsetAsync(largest, 0, 8, s));
     auto pre = dtype == MUZO_BF16 ? attn_bwd_stats_kernel<1> : attn_bwd_stats_kernel<0>;
-    pre<<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const uint16_t*>(out), strides[9], strides[10], strides[11],
-                                                      static_cast<const uint16_t*>(dout), strides[12], strides[13],
-                                                      strides[14], lse, stats, g.hq, seq_q, g.nqt, g.hd, rows);
+    pre<<<static_cast<unsigned>(query_tiles + value_tiles), kStatThreads, 0, s>>>(
+        Rows16{static_cast<const uint16_t*>(out), strides[9], strides[10], strides[11]},
+        Rows16{static_cast<const uint16_t*>(dout), strides[12], strides[13], strides[14]},
+        Rows16{static_cast<const uint16_t*>(v), strides[6], strides[7], strides[8]}, lse, stats, largest, g.hq, seq_q, g.nqt,
+        g.hd, static_cast<unsigned>(query_tiles), g.hkv, seq_k, g.nkt, d_key_lo, d_key_hi);
     st = launch_status();
     if (st != MUZO_OK) return st;
   }

@@ -2,8 +2,9 @@
 keeps for it, against the formulas in 64 bits.
 
 Tolerances are the rounding steps the kernels take, summed worst case with |.| in place of every
-factor: P and dS enter the products rounded to the input type (half a step u = eps / 2, relative,
-and half the smallest subnormal s, absolute), results are rounded once more (u), and fp32 dot
+factor: P and dS enter the products rounded to the input type (half a step u = eps / 2, relative;
+fp16 has subnormals, half a step of which is 2^-25: of 2^10 P, and of dS times the power of two
+that brings 2 max|dO_i| max|v_j| to between 2^14 and 2^15), results are rounded once more (u), and fp32 dot
 products of n terms are off by at most n * 2^-23 of the sum of their terms' magnitudes (2^-16 for the
 128 products of a logit). With autograd, delta = dO . O uses the forward's O, which is rounded (u) and
 took P rounded (u sum P |v|).
@@ -40,7 +41,11 @@ def _exact(q, k, v, dout, scale, vis, out=None):
     O that delta is taken from (otherwise the exact one, whose rounding the bound then counts)."""
     dtype = q.dtype
     u = torch.finfo(dtype).eps / 2
-    s = 2.0 ** -25 if dtype == FP16 else 0.0
+    s_p = s_ds = 0.0
+    if dtype == FP16:
+        s_p = 2.0 ** -35
+        largest = 2 * float(dout.double().norm(dim=-1).max()) * float(torch.nan_to_num(v.double(), 0.0, 0.0, 0.0).norm(dim=-1).max())
+        s_ds = 2.0 ** -25 * max(largest / 2.0 ** 14, 2.0 ** -40)
     b, hq, sq, d = q.shape
     hkv, sk = k.shape[1], k.shape[2]
     group = hq // hkv
@@ -67,13 +72,13 @@ def _exact(q, k, v, dout, scale, vis, out=None):
     if out is None:
         err_delta = err_delta + (ga * (u * used.abs() + (u + 2.0 ** -16) * (p @ va))).sum(-1, keepdim=True)
     err_dp = 2.0 ** -16 * (ga @ va.transpose(2, 3))
-    err_p = p * (rel_p + u) + s * vis
-    err_ds = (ds.abs() * (u + rel_p) + p * (err_dp + err_delta)) * 1.01 + s * vis
+    err_p = p * (rel_p + u) + s_p * vis
+    err_ds = (ds.abs() * (u + rel_p) + p * (err_dp + err_delta)) * 1.01 + s_ds * vis
     n = 2.0 ** -23 * max(sq * group, sk)
     t_dq = ((err_ds + n * ds.abs()) @ ka) * scale + u * dq.abs()
     t_dk = ((err_ds + n * ds.abs()).transpose(2, 3) @ qa * scale).view(b, hkv, group, sk, d).sum(2) + u * dk.abs()
     t_dv = ((err_p + n * p).transpose(2, 3) @ ga).view(b, hkv, group, sk, d).sum(2) + u * dv.abs()
-    extra = 2.0 ** -24 if dtype == FP16 else 0.0     # a result among the subnormals of fp16
+    extra = 2.0 ** -25 if dtype == FP16 else 0.0     # a result among the subnormals of fp16
     return {"out": o.transpose(1, 2), "lse": lse, "dq": dq, "dk": dk, "dv": dv,
             "t_dq": t_dq * 1.05 + 1e-30 + extra, "t_dk": t_dk * 1.05 + 1e-30 + extra, "t_dv": t_dv * 1.05 + 1e-30 + extra}
 
@@ -192,6 +197,27 @@ def test_gradient_against_differences(device, dtype):
         want = (f(plus) - f(minus)) / (2 * h)
         got = float((grads[i].double() * direction).sum())
         assert abs(got - want) <= float((ref["t_" + name] * direction.abs()).sum()) + 1e-6 * (1 + abs(want)), name
+
+
+@pytest.mark.parametrize("gain", [2.0 ** -14, 2.0 ** -6, 2.0 ** 6])
+def test_fp16_small_and_large_gradients(device, gain):
+    """Gradients whose dS would be subnormal in fp16 (or overflow) without its power of two: as exact,
+    relative to the largest result, as ordinary ones. V large too, for the bound's other factor."""
+    from muzo_clip_b200 import attention_max_backward
+    from muzo_clip_b200.attention import _forward
+
+    b, hq, hkv, s, d, scale = 1, 4, 2, 700, 64, 0.125
+    q, k, v, dout = _states(device, FP16, b, hq, hkv, s, s, d, seed=60)
+    dout, v = dout * gain, v * (64.0 if gain > 1 else 1.0)
+    vis = _visible(b, s, s, True, None, None, device)
+    out, lse, _, _ = _forward(q, k, v, scale, True, None, None, False, True)
+    got = attention_max_backward(dout, q, k, v, out, lse, scale, True)
+    ref = _exact(q, k, v, dout, scale, vis, out)
+    _assert_within(got, ref)
+    for g, name in zip(got, ("dq", "dk", "dv")):
+        err = (g.double() - ref[name]).abs()
+        # P, dS and the result rounded: 2^-11 each of terms that sum to less than four times the largest result
+        assert float(err.max()) <= 2.0 ** -9 * float(ref[name].abs().max()) + 2.0 ** -25, name
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
