@@ -1,17 +1,18 @@
 // Attention forward on the tensor cores with the per-head maximum of the pre-softmax logits as a
 // side output: QK-Clip's capture (qk_clip.py:173-196) computed by the attention that the forward
-// runs anyway, so Q K^T is formed once. Forward only (MuZO's forwards run without gradients).
+// runs anyway, so Q K^T is formed once. For training it also keeps each row's log-sum-exp, from which
+// the backward pass (attention_bwd.cu) recomputes the probabilities.
 //
-// One CTA per (batch, query head, block of 256 queries), 11 warps. The block is two query tiles
+// One CTA per (batch, query head, block of 256 queries), 12 warps. The block is two query tiles
 // of 128 rows that share every K / V tile of 128 keys, so each K / V byte loaded serves 256 rows:
 //   warp 0      TMA producer (one thread): both query tiles once, then K tiles (K-major) into a
-//               1-stage ring, refilled once both tiles' S = Q K^T has read it (a stream's next S
-//               waits for its softmax anyway, so the load hides behind the softmax);
+//               1-stage ring, refilled once both tiles' S = Q K^T has read it;
 //   warp 10     TMA producer (one thread): V tiles (MN-major, the second operand of P V) into a
 //               2-stage ring, refilled once both tiles' P V has read it;
-//   warp 1      TMEM owner and MMA issuer (one thread): per query tile s, S_s = Q_s K_j^T into
-//               its S buffer (fp32 in TMEM), then O_s += P_s V_j into its fp32 accumulator, which
-//               stays in TMEM;
+//   warps 1, 11 MMA issuers of query tiles 0 and 1 (one thread each; warp 1 owns TMEM): S_s = Q_s
+//               K_j^T into its S buffer (fp32 in TMEM) as soon as the softmax holds the last S in
+//               registers, so that it is formed while that tile's last exponentials run, then
+//               O_s += P_s V_j into its fp32 accumulator, which stays in TMEM;
 //   warps 2..9  two softmax streams of four warps, stream s for query tile s, one warp per TMEM
 //               lane quarter, one query row per thread, all 128 keys of each tile: the raw
 //               logits' maximum (the side output, over visible logits only), the online softmax
@@ -19,6 +20,9 @@
 //               maximum grows by more than 2^8), P in bf16/fp16 written to shared memory in the
 //               128-byte swizzled K-major layout the MMA reads, and at the end O / l stored to
 //               [B, Sq, Hq, D]. The streams run side by side without waiting for each other.
+// A Llama-3-70B-shaped layer (4096 tokens, 64 and 8 heads of 128, causal) takes 0.355 ms, 775 TFLOP/s:
+// 4700 cycles per K / V tile for both streams, of which 2048 are the special-function unit's, 2048
+// the tensor cores' and 1980 issue, at the GPU's 1000 W.
 // Visibility: key j of batch b is visible to query i when key_lo[b] <= j < key_hi[b] (padding)
 // and, when causal, j <= i + Sk - Sq. Rows without a visible key are written as zeros.
 // Every wait is bounded; on timeout the kernel records a code in the status word, raises its
@@ -133,7 +137,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   // Two query tiles of 128 rows (streams 0 and 1) share every K / V tile of 128 keys: K through a
-  // 2-stage ring (a stage is free once both tiles' S has read it), V through a VS-stage ring (free
+  // K_STAGES ring (a stage is free once both tiles' S has read it), V through a VS-stage ring (free
   // once both tiles' P V has read it). Each stream owns an S buffer and an O accumulator in TMEM
   // and a P tile in shared memory.
   uint8_t* sQ = smem;                                   // [2][NKB][128 x 64]
@@ -191,7 +195,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
   if (warp == 0 || warp == 10) {
     // ------------------------------------------------------------------ TMA producers
-    // warp 0: both query tiles once, then K_j into K stage j % 2 once S_{j-2} of both streams has
+    // warp 0: both query tiles once, then K_j into its stage once S_{j - K_STAGES} of both streams has
     // read it; warp 10: V_j into V stage j % VS once P_{j-VS} V_{j-VS} of both streams has read it
     if (lane == 0 && ntiles > 0) {
       const bool keys = warp == 0;

@@ -79,6 +79,7 @@ Tensor attention_status(int device) {
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     const auto options = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device);
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+      c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
       c10::cuda::CUDAStreamGuard side(c10::cuda::getStreamFromPool(false, static_cast<c10::DeviceIndex>(device)));
       t = at::zeros({2}, options);
     } else {

@@ -454,6 +454,106 @@ def test_backward_bounded_waits_expire(device, role):
     assert all(torch.equal(a, c) for a, c in zip(got, want))
 
 
+def test_ranges_beyond_the_sequence(device):
+    """key_lo below 0 or behind the keys, key_hi behind them or negative: clamped, or nothing is seen."""
+    from muzo_clip_b200 import attention_max
+
+    b, hq, hkv, s, d = 4, 4, 2, 200, 64
+    q, k, v, dout = _states(device, BF16, b, hq, hkv, s, s, d, seed=41)
+    big = 2 ** 31 - 1
+
+    def run(lo, hi):
+        leaves = [x.detach().clone().requires_grad_(True) for x in (q, k, v)]
+        out, smax, valid = attention_max(*leaves, None, False, *_range(device, b, lo, hi))
+        return [out.detach(), smax, *torch.autograd.grad(out, leaves, dout)]
+
+    for a, c in zip(run([-5, 0, big, 3], [big, s, big, -7]), run([0, 0, s, 3], [s, s, s, 3])):
+        assert torch.equal(a, c)
+    got = run([-5, 0, big, 3], [big, s, big, -7])
+    assert not any(bool(g[2:].any()) for g in (got[0], *got[2:]))
+
+
+def test_one_tensor_as_query_key_and_value(device):
+    """The gradients of one leaf in three places add up."""
+    from muzo_clip_b200 import attention_max
+
+    x, _, _, dout = _states(device, BF16, 2, 2, 2, 150, 150, 64, seed=42)
+    one = x.detach().clone().requires_grad_(True)
+    attention_max(one, one, one)[0].backward(dout)
+    three = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    attention_max(*three)[0].backward(dout)
+    # autograd adds the three in bf16, in an order of its own: two more roundings
+    want = sum(t.grad.double() for t in three)
+    size = sum(t.grad.double().abs() for t in three)
+    assert bool(((one.grad.double() - want).abs() <= 2 * 2.0 ** -8 * size).all())
+
+
+def test_differentiable_once(device):
+    from muzo_clip_b200 import attention_max
+
+    q, k, v, dout = _states(device, BF16, 1, 2, 2, 50, 50, 64, seed=43)
+    leaves = [x.detach().clone().requires_grad_(True) for x in (q, k, v)]
+    out, smax, _ = attention_max(*leaves)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, leaves, dout, create_graph=True)
+    with torch.no_grad():
+        assert not attention_max(*leaves)[0].requires_grad
+
+
+@pytest.mark.parametrize("sq,sk", [(270001, 33), (33, 270001)])
+def test_offsets_beyond_32_bits(device, sq, sk):
+    """More than 2^31 elements of queries, or of keys: the last head's last rows, in a batch of one
+    with 64 heads, against the formulas on that head alone."""
+    from muzo_clip_b200 import attention_max_backward
+    from muzo_clip_b200.attention import _forward
+
+    h, d = 64, 128
+    gen = torch.Generator(device=device).manual_seed(3)
+
+    def x(s):
+        return torch.randn((1, s, h, d), generator=gen, device=device, dtype=BF16).transpose(1, 2)
+
+    q, k, v, dout = x(sq), x(sk), x(sk), x(sq).transpose(1, 2)
+    assert max(q.numel(), k.numel()) > 2 ** 31
+    out, lse, _, _ = _forward(q, k, v, 0.05, False, None, None, False, True)
+    got = attention_max_backward(dout, q, k, v, out, lse, 0.05, False)
+    sub = [t[:, -1:] for t in (q, k, v)] + [dout[:, :, -1:]]
+    ref = _exact(*sub, 0.05, torch.ones((1, 1, sq, sk), dtype=torch.bool, device=device), out[:, :, -1:])
+    _assert_within([g[:, -1:] for g in got], ref)
+
+
+def test_first_call_of_a_process_is_captured():
+    """A process whose first attention call is being captured: the status words, the kernels' attributes
+    and the modules are set up under capture, and the replay computes what an eager call does."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = f"""
+import sys; sys.path.insert(0, {str(ROOT / "muzo-clip_b200")!r})
+import torch
+from muzo_clip_b200 import attention_max, clip_grads
+g = torch.Generator(device="cuda").manual_seed(0)
+x = [torch.randn((1, 4, 200, 64), generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+def run():
+    leaves = [t.detach().requires_grad_(True) for t in x]
+    out, smax, valid = attention_max(*leaves)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    scaled, norm = clip_grads(list(grads), 0.5)
+    return [out.detach(), smax, valid, *grads, *scaled, norm]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+print("the same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stdout + done.stderr
+
+
 def test_refusals(device):
     from muzo_clip_b200 import attention_max, attention_max_backward
 
