@@ -340,19 +340,62 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int stall = *reinterpret_cast<volatile int*>(g.status + 1);
   const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
 
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
     // arrivals: the eight probability warps on kP and kDs, the warp that waits for a key CTA's loads on its second
     // kP, a query CTA's two issuers on kDone
-    for (int i = 0; i < kBars; ++i)
+    static_assert(kBars <= 32, "one lane per barrier");
+    const int i = lane;
+    if (i < kBars)
       mbar_init(bars + i, i == kP + 1 ? 9 : (i >= kP && i < kDone ? 8 : (i == kDone && !key_cta ? 2 : 1)));
-    *abort_flag = 0;
+    if (lane == 0) *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                  "r"(B_TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // The CTA's work, and the producer's first loads: they run while the others still wait for TMEM.
+  Armed armed;
+  int kt = 0, qt_own = 0, b, bh_own, first, count, begin = 0, n;
+  int64_t lo, hi;
+  if (key_cta) {
+    const unsigned per_tile = static_cast<unsigned>(g.batch * g.hkv * g.parts);
+    kt = static_cast<int>(blockIdx.x / per_tile);   // causal: the first key tiles see the most queries
+    const unsigned rest = blockIdx.x % per_tile;
+    const int part = static_cast<int>(rest % g.parts);
+    bh_own = static_cast<int>(rest / g.parts);
+    b = bh_own / g.hkv;
+    key_tile_queries(g, b, kt, lo, hi, first, count);
+    // this CTA's share of the (head, query tile) pairs
+    const int total = g.group * count;
+    const int chunk = (total + g.parts - 1) / g.parts;
+    begin = part * chunk < total ? part * chunk : total;
+    n = (begin + chunk < total ? begin + chunk : total) - begin;
+  } else {
+    const unsigned item = blockIdx.x - static_cast<unsigned>(g.key_items);
+    const unsigned bh_count = static_cast<unsigned>(g.batch * g.hq);
+    qt_own = g.nqt - 1 - static_cast<int>(item / bh_count);   // causal: the last query tiles see the most keys
+    bh_own = static_cast<int>(item % bh_count);
+    b = bh_own / g.hq;
+    query_tile_keys(g, b, qt_own, lo, hi, first, n);
+    count = n;
+  }
+  if (threadIdx.x == 0 && n > 0) {
+    if (key_cta) {
+      armed.arm(bars, 0, 0, TILE);
+      load_tile<NKB>(&map_k, bars + kFull, smem, kt * AN, bh_own % g.hkv, b);
+      armed.arm(bars, 1, 0, TILE);
+      load_tile<NKB>(&map_v, bars + kFull + 1, smem + TILE, kt * AN, bh_own % g.hkv, b);
+    } else {
+      const int h = bh_own % g.hq;
+      armed.arm(bars, 0, 0, TILE);
+      load_tile<NKB>(&map_q, bars + kFull, smem, qt_own * AM, h, b);
+      armed.arm(bars, 1, 0, TILE);
+      load_tile<NKB>(&map_do, bars + kFull + 1, smem + TILE, qt_own * AM, h, b);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -366,20 +409,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   if (key_cta) {
     // ================================================================ 128 keys: dK, dV
-    const int64_t per_tile = static_cast<int64_t>(g.batch) * g.hkv * g.parts;
-    const int kt = static_cast<int>(blockIdx.x / per_tile);   // causal: the first key tiles see the most queries
-    const int64_t rest = blockIdx.x % per_tile;
-    const int part = static_cast<int>(rest % g.parts);
-    const int bh = static_cast<int>(rest / g.parts);
-    const int b = bh / g.hkv, kvh = bh % g.hkv;
-    int64_t lo, hi;
-    int first, count;
-    key_tile_queries(g, b, kt, lo, hi, first, count);
-    // this CTA's share of the (head, query tile) pairs
-    const int total = g.group * count;
-    const int chunk = (total + g.parts - 1) / g.parts;
-    const int begin = part * chunk < total ? part * chunk : total;
-    const int n = (begin + chunk < total ? begin + chunk : total) - begin;
+    const int bh = bh_own, kvh = bh % g.hkv;
+    const int part = static_cast<int>(blockIdx.x % static_cast<unsigned>(g.parts));
     uint8_t* sK = smem;
     uint8_t* sV = smem + TILE;
     uint8_t* sQ = smem + 2 * TILE;        // 3 stages
@@ -390,27 +421,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     if (warp == 0) {
       if (lane == 0 && n > 0) {
-        Armed armed;
         bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
         for (int t = 0; t < n && ok; ++t) {
           const int sq = t % 3, so = t & 1;
           const uint32_t pq = (t / 3) & 1, po = (t >> 1) & 1;
           const int head = kvh * g.group + (begin + t) / count, qt = first + (begin + t) % count;
           const float* st = g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256;
-          if (t == 0) {
-            armed.arm(bars, 0, 0, TILE);
-            load_tile<NKB>(&map_k, bars + kFull, sK, kt * AN, kvh, b);
-          }
           // a Q stage is free after its dK, a dO stage after its dV (issued behind dP)
           if (!wait_one<false>(bars + kEmpty + 2 + sq, pq ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 2 + sq, pq, TILE + 512);
           load_tile<NKB>(&map_q, bars + kFull + 2 + sq, sQ + sq * TILE, qt * AM, head, b);
           if (t == 0) wait_for_statistics();
           bulk_load(delta + sq * 128, st + 128, 512, bars + kFull + 2 + sq);
-          if (t == 0) {
-            armed.arm(bars, 1, 0, TILE);
-            load_tile<NKB>(&map_v, bars + kFull + 1, sV, kt * AN, kvh, b);
-          }
           if (!wait_one<false>(bars + kEmpty + 5 + so, po ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 5 + so, po, TILE + 512);
           bulk_load(neg_lse + so * 128, st, 512, bars + kFull + 5 + so);
@@ -610,14 +632,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
   } else {
     // ================================================================ 128 queries: dQ
-    const int64_t item = static_cast<int64_t>(blockIdx.x) - g.key_items;
-    const int64_t bh_count = static_cast<int64_t>(g.batch) * g.hq;
-    const int qt = g.nqt - 1 - static_cast<int>(item / bh_count);   // causal: the last query tiles see the most keys
-    const int64_t bh = item % bh_count;
-    const int b = static_cast<int>(bh / g.hq), h = static_cast<int>(bh % g.hq), kvh = h / g.group;
-    int64_t lo, hi;
-    int first, n;
-    query_tile_keys(g, b, qt, lo, hi, first, n);
+    const int qt = qt_own, h = bh_own % g.hq, kvh = h / g.group;
+    const int64_t bh = bh_own;
     uint8_t* sQ = smem;
     uint8_t* sO = smem + TILE;
     uint8_t* sK = smem + 2 * TILE;    // 3 stages
@@ -626,23 +642,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     if (warp == 0) {
       if (lane == 0 && n > 0) {
-        Armed armed;
         bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
         for (int t = 0; t < n && ok; ++t) {
           const int sk_ = t % 3, sv_ = t & 1;
           const uint32_t pk = (t / 3) & 1, pv = (t >> 1) & 1;
           const int row = (first + t) * AN;
-          if (t == 0) {
-            armed.arm(bars, 0, 0, TILE);
-            load_tile<NKB>(&map_q, bars + kFull, sQ, qt * AM, h, b);
-          }
           if (!wait_one<false>(bars + kEmpty + 2 + sk_, pk ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 2 + sk_, pk, TILE);
           load_tile<NKB>(&map_k, bars + kFull + 2 + sk_, sK + sk_ * TILE, row, kvh, b);
-          if (t == 0) {
-            armed.arm(bars, 1, 0, TILE);
-            load_tile<NKB>(&map_do, bars + kFull + 1, sO, qt * AM, h, b);
-          }
           if (!wait_one<false>(bars + kEmpty + 5 + sv_, pv ^ 1, abort_flag)) { ok = false; break; }
           armed.arm(bars, 5 + sv_, pv, TILE);
           load_tile<NKB>(&map_v, bars + kFull + 5 + sv_, sV + sv_ * TILE, row, kvh, b);
