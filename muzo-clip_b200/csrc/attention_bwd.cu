@@ -865,44 +865,55 @@ attn_bwd_stats_kernel(Rows16 o, Rows16 d, Rows16 v, const float* lse, float* sta
     const int bh = static_cast<int>(t / nkt), kt = static_cast<int>(t % nkt), b = bh / hkv;
     int64_t lo, hi;
     key_range(key_lo, key_hi, sk, b, lo, hi);
-    const uint16_t* base = v.p + b * v.sb + (bh % hkv) * v.sh + 8 * l;
+    const uint16_t* base = v.p + b * v.sb + (bh % hkv) * v.sh + (here ? 8 * l : 0);
+    float x[AM / kStatGroups][8];
 #pragma unroll
     for (int r = 0; r < AM / kStatGroups; ++r) {
       const int64_t j = static_cast<int64_t>(kt) * AN + kStatGroups * r + group;
-      float x[8] = {}, s = 0.0f;
-      if (here && j >= lo && j < hi) load8(base, j * v.ss, type, x);
+      load8(base, (j < sk ? j : sk - 1) * v.ss, type, x[r]);
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(x[e], x[e], s);
-      square = larger(square, sum16(s));
+    for (int r = 0; r < AM / kStatGroups; ++r) {
+      const int64_t j = static_cast<int64_t>(kt) * AN + kStatGroups * r + group;
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf(x[r][e], x[r][e], s);
+      square = larger(square, sum16(here && j >= lo && j < hi ? s : 0.0f));
     }
     block_largest(square, largest + 1);
     return;
   }
   const int bh = static_cast<int>(blockIdx.x / nqt), qt = static_cast<int>(blockIdx.x % nqt), b = bh / hq, h = bh % hq;
-  const uint16_t* ob = o.p + b * o.sb + h * o.sh + 8 * l;
-  const uint16_t* db = d.p + b * d.sb + h * d.sh + 8 * l;
+  const int64_t col = here ? 8 * l : 0;
+  const uint16_t* ob = o.p + b * o.sb + h * o.sh + col;
+  const uint16_t* db = d.p + b * d.sb + h * d.sh + col;
   float* tile = stats + static_cast<int64_t>(blockIdx.x) * 256;
+  constexpr int R = AM / kStatGroups;
+  // every load is issued before the first is used (lanes and rows that do not exist read one that does)
+  float x[R][8], y[R][8], w[R];
 #pragma unroll
-  for (int r = 0; r < AM / kStatGroups; ++r) {
+  for (int r = 0; r < R; ++r) {
+    const int64_t i = static_cast<int64_t>(qt) * AM + kStatGroups * r + group;
+    const int64_t at = i < sq ? i : sq - 1;
+    load8(ob, at * o.ss, type, x[r]);
+    load8(db, at * d.ss, type, y[r]);
+    w[r] = l == 0 && i < sq ? lse[static_cast<int64_t>(bh) * sq + i] : -INFINITY;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
     const int row = kStatGroups * r + group;
-    const int64_t i = static_cast<int64_t>(qt) * AM + row;
-    const bool in = i < sq;
-    float x[8] = {}, y[8] = {}, sum = 0.0f, s = 0.0f;
-    if (here && in) {
-      load8(ob, i * o.ss, type, x);
-      load8(db, i * d.ss, type, y);
-    }
+    const bool in = static_cast<int64_t>(qt) * AM + row < sq;
+    float sum = 0.0f, s = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      sum = fmaf(x[e], y[e], sum);
-      if (FMT == 0) s = fmaf(y[e], y[e], s);
+      sum = fmaf(x[r][e], y[r][e], sum);
+      if (FMT == 0) s = fmaf(y[r][e], y[r][e], s);
     }
-    sum = sum16(sum);
-    if (FMT == 0) square = larger(square, sum16(s));
+    sum = sum16(here && in ? sum : 0.0f);
+    if (FMT == 0) square = larger(square, sum16(here && in ? s : 0.0f));
     if (l == 0) {
-      const float w = in ? lse[static_cast<int64_t>(bh) * sq + i] : -INFINITY;
-      tile[row] = w == -INFINITY ? -INFINITY : fmaf(-w, kLog2e, FMT == 0 ? 10.0f : 0.0f);   // fp16: 2^10 P
-      tile[128 + row] = in ? sum : 0.0f;
+      tile[row] = w[r] == -INFINITY ? -INFINITY : fmaf(-w[r], kLog2e, FMT == 0 ? 10.0f : 0.0f);   // fp16: 2^10 P
+      tile[128 + row] = sum;
     }
   }
   if (FMT == 0) block_largest(square, largest);
