@@ -705,6 +705,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       wait_for_statistics();
       const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
       const float nl = n > 0 ? st[r] : 0.0f, delta = n > 0 ? st[128 + r] : 0.0f;
+      const float delta_ds = -delta * two.ds;
       int64_t end = hi;                                      // visible keys of this row: [lo, end)
       if (g.causal && row + g.shift + 1 < end) end = row + g.shift + 1;
       if (!row_in) end = lo;
@@ -745,7 +746,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (lane == 0) mbar_arrive(bars + kP);   // dP(t) read: the next one may be formed
           s_here = look(bars + kS + ((t + 1) & 1), ((t + 1) >> 1) & 1);
 #pragma unroll
-          for (int c = 0; c < 64; ++c) p[c] *= scaled_less<FMT>(v[c], delta, two.ds);
+          for (int c = 0; c < 64; ++c)
+            p[c] *= FMT == 1 ? __uint_as_float(v[c]) - delta : fmaf(__uint_as_float(v[c]), two.ds, delta_ds);
         }
         if (!all_seen) {   // a masked pair's dP may be anything (V of a key outside the range)
 #pragma unroll
