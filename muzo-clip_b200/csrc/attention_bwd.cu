@@ -383,18 +383,39 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     query_tile_keys(g, b, qt_own, lo, hi, first, n);
     count = n;
   }
+  // A key CTA's tile t: one Q stage with delta, one dO stage with -lse, as the buffers below are laid out.
+  auto load_query_tile = [&](int t, bool q_part, uint32_t phase) {
+    const int pair = begin + t, head = (bh_own % g.hkv) * g.group + pair / count, qt = first + pair % count;
+    const float* st = g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256;
+    float* stat_base = reinterpret_cast<float*>(smem + L::TILES * TILE);   // delta [3][128], -lse [2][128]
+    const int s = q_part ? t % 3 : t & 1, bar = (q_part ? 2 : 5) + s;
+    armed.arm(bars, bar, phase, TILE + 512);
+    load_tile<NKB>(q_part ? &map_q : &map_do, bars + kFull + bar, smem + bar * TILE, qt * AM, head, b);
+    if (t == 0) wait_for_statistics();
+    bulk_load(stat_base + (q_part ? s : 3 + s) * 128, q_part ? st + 128 : st, 512, bars + kFull + bar);
+  };
+  // A query CTA's key tile t: a K or a V stage.
+  auto load_key_tile = [&](int t, bool k_part, uint32_t phase) {
+    const int bar = k_part ? 2 + t % 3 : 5 + (t & 1);
+    armed.arm(bars, bar, phase, TILE);
+    load_tile<NKB>(k_part ? &map_k : &map_v, bars + kFull + bar, smem + bar * TILE, (first + t) * AN,
+                   (bh_own % g.hq) / g.group, b);
+  };
+  auto load_own = [&](const CUtensorMap* map, int bar, int row, int head) {
+    armed.arm(bars, bar, 0, TILE);
+    load_tile<NKB>(map, bars + kFull + bar, smem + bar * TILE, row, head, b);
+  };
   if (threadIdx.x == 0 && n > 0) {
     if (key_cta) {
-      armed.arm(bars, 0, 0, TILE);
-      load_tile<NKB>(&map_k, bars + kFull, smem, kt * AN, bh_own % g.hkv, b);
-      armed.arm(bars, 1, 0, TILE);
-      load_tile<NKB>(&map_v, bars + kFull + 1, smem + TILE, kt * AN, bh_own % g.hkv, b);
+      load_own(&map_k, 0, kt * AN, bh_own % g.hkv);
+      load_query_tile(0, true, 0);
+      load_own(&map_v, 1, kt * AN, bh_own % g.hkv);
+      load_query_tile(0, false, 0);
     } else {
-      const int h = bh_own % g.hq;
-      armed.arm(bars, 0, 0, TILE);
-      load_tile<NKB>(&map_q, bars + kFull, smem, qt_own * AM, h, b);
-      armed.arm(bars, 1, 0, TILE);
-      load_tile<NKB>(&map_do, bars + kFull + 1, smem + TILE, qt_own * AM, h, b);
+      load_own(&map_q, 0, qt_own * AM, bh_own % g.hq);
+      load_key_tile(0, true, 0);
+      load_own(&map_do, 1, qt_own * AM, bh_own % g.hq);
+      load_key_tile(0, false, 0);
     }
   }
   tc_fence_before();
@@ -422,21 +443,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (warp == 0) {
       if (lane == 0 && n > 0) {
         bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
-        for (int t = 0; t < n && ok; ++t) {
+        for (int t = 1; t < n && ok; ++t) {   // a Q stage is free after its dK, a dO stage after its dV (issued behind dP)
           const int sq = t % 3, so = t & 1;
           const uint32_t pq = (t / 3) & 1, po = (t >> 1) & 1;
-          const int head = kvh * g.group + (begin + t) / count, qt = first + (begin + t) % count;
-          const float* st = g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256;
-          // a Q stage is free after its dK, a dO stage after its dV (issued behind dP)
-          if (!wait_one<false>(bars + kEmpty + 2 + sq, pq ^ 1, abort_flag)) { ok = false; break; }
-          armed.arm(bars, 2 + sq, pq, TILE + 512);
-          load_tile<NKB>(&map_q, bars + kFull + 2 + sq, sQ + sq * TILE, qt * AM, head, b);
-          if (t == 0) wait_for_statistics();
-          bulk_load(delta + sq * 128, st + 128, 512, bars + kFull + 2 + sq);
-          if (!wait_one<false>(bars + kEmpty + 5 + so, po ^ 1, abort_flag)) { ok = false; break; }
-          armed.arm(bars, 5 + so, po, TILE + 512);
-          bulk_load(neg_lse + so * 128, st, 512, bars + kFull + 5 + so);
-          load_tile<NKB>(&map_do, bars + kFull + 5 + so, sO + so * TILE, qt * AM, head, b);
+          ok = wait_one<false>(bars + kEmpty + 2 + sq, pq ^ 1, abort_flag);
+          if (ok) load_query_tile(t, true, pq);
+          ok = ok && wait_one<false>(bars + kEmpty + 5 + so, po ^ 1, abort_flag);
+          if (ok) load_query_tile(t, false, po);
         }
         if (!ok) give_up(g, abort_flag, kErrTimeoutProducer);
         armed.wait_all(bars);   // every load of this CTA has landed before it may exit (bounded)
@@ -643,16 +656,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (warp == 0) {
       if (lane == 0 && n > 0) {
         bool ok = stall != kErrTimeoutProducer || mbar_wait(bars + kStall, 0, kStallLimitCycles);
-        for (int t = 0; t < n && ok; ++t) {
-          const int sk_ = t % 3, sv_ = t & 1;
+        for (int t = 1; t < n && ok; ++t) {
           const uint32_t pk = (t / 3) & 1, pv = (t >> 1) & 1;
-          const int row = (first + t) * AN;
-          if (!wait_one<false>(bars + kEmpty + 2 + sk_, pk ^ 1, abort_flag)) { ok = false; break; }
-          armed.arm(bars, 2 + sk_, pk, TILE);
-          load_tile<NKB>(&map_k, bars + kFull + 2 + sk_, sK + sk_ * TILE, row, kvh, b);
-          if (!wait_one<false>(bars + kEmpty + 5 + sv_, pv ^ 1, abort_flag)) { ok = false; break; }
-          armed.arm(bars, 5 + sv_, pv, TILE);
-          load_tile<NKB>(&map_v, bars + kFull + 5 + sv_, sV + sv_ * TILE, row, kvh, b);
+          ok = wait_one<false>(bars + kEmpty + 2 + t % 3, pk ^ 1, abort_flag);
+          if (ok) load_key_tile(t, true, pk);
+          ok = ok && wait_one<false>(bars + kEmpty + 5 + (t & 1), pv ^ 1, abort_flag);
+          if (ok) load_key_tile(t, false, pv);
         }
         if (!ok) give_up(g, abort_flag, kErrTimeoutProducer);
         armed.wait_all(bars);
