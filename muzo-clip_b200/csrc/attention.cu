@@ -114,6 +114,21 @@ __device__ __forceinline__ void attn_tiles(const AttnArgs& g, int b, int qb, int
   n1 = n[1];
 }
 
+// The two softmax streams take turns at their exponentials: one fills the special-function unit while
+// the other takes its tile's maximum and waits for its products. Without turns both did the same at
+// the same time (4300 cycles a tile for both, 2050 of them the unit's). Stream 0 waits from its second
+// tile on for stream 1's last tile, stream 1 for stream 0's same tile; where the other stream has no
+// such tile there is nothing to wait for. Both streams execute every turn, after a timeout too, so the
+// hardware barriers (which have no time limit) always complete.
+constexpr int kTurnBarrier = 1;   // named barriers 1 (stream 0's turn) and 2
+__device__ __forceinline__ void turn_wait(int stream, int u, int n0, int n1) {
+  if (stream == 0 ? (u >= 1 && u - 1 < n1) : u < n0)
+    asm volatile("bar.sync %0, 256;" ::"r"(kTurnBarrier + stream) : "memory");
+}
+__device__ __forceinline__ void turn_pass(int stream, int u, int n0, int n1) {
+  if (stream == 0 ? u < n1 : u + 1 < n0) asm volatile("bar.arrive %0, 256;" ::"r"(kTurnBarrier + 1 - stream) : "memory");
+}
+
 // Three-input maximum (NaN-propagating) and minimum (sm_100).
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
@@ -341,6 +356,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (lane == 0) waited = mbar_wait(stall_bar, 0, kStallLimitCycles);
       ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
     }
+    int turns = 0;   // turns taken and passed on
     for (int u = 0; u < n_mine && ok; ++u) {
       bool ready = true;
       if (lane == 0) ready = mbar_wait(s_full + stream, static_cast<uint32_t>(u & 1));
@@ -420,6 +436,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       }
       // pass 2: P = 2^(s * scale_log2 - m_run), its row sum, and P in the 128-byte swizzled K-major
       // layout (chunk c16 of 8 keys of K block ch sits at row * 128 + ((c16 ^ (row & 7)) * 16))
+      turn_wait(stream, u, n0, n1);
       const float nm = -m_run;
       float lsum[8];
 #pragma unroll
@@ -466,6 +483,8 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
               make_uint4(packed[4 * c16], packed[4 * c16 + 1], packed[4 * c16 + 2], packed[4 * c16 + 3]);
         }
       }
+      turn_pass(stream, u, n0, n1);
+      turns = u + 1;
       l_run = l_run * alpha + (((lsum[0] + lsum[1]) + (lsum[2] + lsum[3])) + ((lsum[4] + lsum[5]) + (lsum[6] + lsum[7])));
       // keys outside [lo, hi) that share a tile with visible ones: their P is 0, but 0 times a
       // non-finite V would still reach O, so their V rows are cleared before P V reads them
@@ -487,6 +506,10 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + stream);
+    }
+    for (; turns < n_mine; ++turns) {   // this warp gave up: its turns pass all the same
+      turn_wait(stream, turns, n0, n1);
+      turn_pass(stream, turns, n0, n1);
     }
     // this stream's last P V must be done before O_s is read
     if (ok && n_mine > 0) {
