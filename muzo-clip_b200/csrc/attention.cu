@@ -11,7 +11,7 @@
 //               2-stage ring, refilled once both tiles' P V has read it;
 //   warps 1, 11 MMA issuers of query tiles 0 and 1 (one thread each; warp 1 owns TMEM): S_s = Q_s
 //               K_j^T into its S buffer (fp32 in TMEM) as soon as the softmax holds the last S in
-//               registers, so that it is formed while that tile's last exponentials run, then
+//               registers, so that it is formed while that tile's exponentials run, then
 //               O_s += P_s V_j into its fp32 accumulator, which stays in TMEM;
 //   warps 2..9  two softmax streams of four warps, stream s for query tile s, one warp per TMEM
 //               lane quarter, one query row per thread, all 128 keys of each tile: the raw
@@ -19,10 +19,13 @@
 //               in base 2 with a lazy rescale (O and the row sum are rescaled only when the row
 //               maximum grows by more than 2^8), P in bf16/fp16 written to shared memory in the
 //               128-byte swizzled K-major layout the MMA reads, and at the end O / l stored to
-//               [B, Sq, Hq, D]. The streams run side by side without waiting for each other.
-// A Llama-3-70B-shaped layer (4096 tokens, 64 and 8 heads of 128, causal) takes 0.355 ms, 775 TFLOP/s:
-// 4700 cycles per K / V tile for both streams, of which 2048 are the special-function unit's, 2048
-// the tensor cores' and 1980 issue, at the GPU's 1000 W.
+//               [B, Sq, Hq, D]. The streams take turns at their exponentials: one has the
+//               special-function unit to itself while the other waits for its S, finds its maxima
+//               and hands its P over.
+// A Llama-3-70B-shaped layer (4096 tokens, 64 and 8 heads of 128, causal) takes 0.269 ms, 1020 TFLOP/s:
+// about 3400 cycles per K / V tile for both streams, of which 2048 are the special-function unit's and
+// 2048 the tensor cores'. A turn takes 1500 cycles, not 1024, one warp per scheduler being all that
+// issues in it, and its hand-over 150.
 // Visibility: key j of batch b is visible to query i when key_lo[b] <= j < key_hi[b] (padding)
 // and, when causal, j <= i + Sk - Sq. Rows without a visible key are written as zeros.
 // Every wait is bounded; on timeout the kernel records a code in the status word, raises its
@@ -374,31 +377,31 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (c_hi < c_lo) c_hi = c_lo;
       }
       const bool all_visible = c_lo == 0 && c_hi == AN;
-      // pass 1: the tile's maximum (and, to record, minimum) over the visible logits
+      // S into registers, once: the columns are free for the next S while this tile's exponentials
+      // run. 128 of the thread's 168 registers hold the row (both passes reading TMEM instead:
+      // 314 us against 286 for a Llama-3-70B-shaped layer).
+      uint32_t v[AN];
+      tmem_ld128(s_cols, v);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free + stream);
+      // the tile's maximum (and, to record, minimum) over the visible logits; the others become -inf
       float mx[4], mn[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) { mx[q] = -INFINITY; mn[q] = INFINITY; }
+      if (!all_visible) {
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t v[64];
-        tmem_ld64(s_cols + ch * 64, v);
-        if (all_visible) {
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
-            mx[(c >> 1) & 3] = max3_nan(mx[(c >> 1) & 3], x0, x1);
-            if (REC) mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], x0, x1);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const int k0 = ch * 64 + c;
-            const bool v0 = k0 >= c_lo && k0 < c_hi, v1 = k0 + 1 >= c_lo && k0 + 1 < c_hi;
-            const float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
-            mx[(c >> 1) & 3] = max3_nan(mx[(c >> 1) & 3], v0 ? x0 : -INFINITY, v1 ? x1 : -INFINITY);
-            if (REC) mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], v0 ? x0 : INFINITY, v1 ? x1 : INFINITY);
-          }
+        for (int c = 0; c < AN; ++c) {
+          const bool visible = c >= c_lo && c < c_hi;
+          if (REC) mn[c & 3] = fminf(mn[c & 3], visible ? __uint_as_float(v[c]) : INFINITY);
+          if (!visible) v[c] = 0xff800000u;
         }
+      }
+#pragma unroll
+      for (int c = 0; c < AN; c += 2) {
+        const float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
+        mx[(c >> 1) & 3] = max3_nan(mx[(c >> 1) & 3], x0, x1);
+        if (REC && all_visible) mn[(c >> 1) & 3] = min3(mn[(c >> 1) & 3], x0, x1);
       }
       const float mt = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
       if (REC) {
@@ -424,64 +427,38 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       }
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld32(o_cols + c * 32, v);
+        for (int c = 0; c < D / 16; ++c) {   // 16 at a time: S holds most of the registers
+          uint32_t o[16];
+          tmem_ld16(o_cols + c * 16, o);
           if (rescale) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
           }
-          tmem_st32(o_cols + c * 32, v);
+          tmem_st16(o_cols + c * 16, o);
         }
       }
-      // pass 2: P = 2^(s * scale_log2 - m_run), its row sum, and P in the 128-byte swizzled K-major
-      // layout (chunk c16 of 8 keys of K block ch sits at row * 128 + ((c16 ^ (row & 7)) * 16))
+      // P = 2^(s * scale_log2 - m_run), its row sum, and P in the 128-byte swizzled K-major layout
+      // (chunk c16 of 8 keys of K block c16 / 8 sits at row * 128 + ((c16 ^ (row & 7)) * 16, modulo 8).
+      // A row that has seen no logit above -inf has all of this tile's there: 1 * -inf + 0 gives P = 0.
+      const float nm = m_run == -INFINITY ? 0.0f : -m_run, mul = m_run == -INFINITY ? 1.0f : g.scale_log2;
       turn_wait(stream, u, n0, n1);
-      const float nm = -m_run;
       float lsum[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) lsum[q] = 0.0f;
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        uint32_t v[64];
-        tmem_ld64(s_cols + ch * 64, v);
-        if (ch == 1) {   // S is read: the next one may be formed while this tile's exponentials run
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free + stream);
+      for (int c16 = 0; c16 < AN / 8; ++c16) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 8 * c16 + 2 * e;
+          float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
+          fma_pair(x0, x1, mul, nm);
+          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+          add_pair(lsum[2 * e], lsum[2 * e + 1], p0, p1);
+          w[e] = FMT == 1 ? pack_bf16(p0, p1) : pack_half(p0, p1);
         }
-        uint32_t packed[32];
-        if (m_run == -INFINITY) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) packed[c] = 0u;
-        } else if (all_visible) {
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nm));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(v[c + 1]), g.scale_log2, nm));
-            lsum[(c >> 1) & 3] += p0;
-            lsum[((c >> 1) & 3) + 4] += p1;
-            packed[c >> 1] = FMT == 1 ? pack_bf16(p0, p1) : pack_half(p0, p1);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const int k0 = ch * 64 + c;
-            const float x0 = (k0 >= c_lo && k0 < c_hi) ? __uint_as_float(v[c]) : -INFINITY;
-            const float x1 = (k0 + 1 >= c_lo && k0 + 1 < c_hi) ? __uint_as_float(v[c + 1]) : -INFINITY;
-            const float p0 = fast_exp2(fmaf(x0, g.scale_log2, nm));
-            const float p1 = fast_exp2(fmaf(x1, g.scale_log2, nm));
-            lsum[(c >> 1) & 3] += p0;
-            lsum[((c >> 1) & 3) + 4] += p1;
-            packed[c >> 1] = FMT == 1 ? pack_bf16(p0, p1) : pack_half(p0, p1);
-          }
-        }
-#pragma unroll
-        for (int c16 = 0; c16 < 8; ++c16) {
-          uint8_t* dst = my_p + ch * SUB_BYTES + r * 128 + ((c16 ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(dst) =
-              make_uint4(packed[4 * c16], packed[4 * c16 + 1], packed[4 * c16 + 2], packed[4 * c16 + 3]);
-        }
+        *reinterpret_cast<uint4*>(my_p + (c16 >> 3) * SUB_BYTES + r * 128 + (((c16 ^ r) & 7) << 4)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
       }
       turn_pass(stream, u, n0, n1);
       turns = u + 1;

@@ -18,6 +18,28 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Two fp32 values in one instruction of the FMA pipe, each rounded once as its scalar form is:
+// x = x * a + b, and x += y.
+__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a, float b) {
+  asm("{\n\t.reg .b64 x, a, b;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 a, {%2, %2};\n\t"
+      "mov.b64 b, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, a, b;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add_pair(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y0), "f"(y1));
+}
+
 // Visible keys [lo, hi) of batch row b, clamped to the sequence.
 __device__ __forceinline__ void key_range(const int32_t* key_lo, const int32_t* key_hi, int64_t sk, int b, int64_t& lo,
                                           int64_t& hi) {
