@@ -452,7 +452,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         for (int e = 0; e < 4; ++e) {
           const int c = 8 * c16 + 2 * e;
           float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
-          fma_pair(x0, x1, mul, nm);
+          fma_pair(x0, x1, mul, nm, nm);
           const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
           add_pair(lsum[2 * e], lsum[2 * e + 1], p0, p1);
           w[e] = FMT == 1 ? pack_bf16(p0, p1) : pack_half(p0, p1);

@@ -17,13 +17,13 @@
 // TMEM, over the columns of the S and dP they came from, so shared memory holds operand tiles only (three
 // Q and two dO stages, or three K and two V stages, beside the resident pair).
 //
-// What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1140 cycles, of
-// which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2800 cycles with
+// What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1100 cycles, of
+// which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2700 cycles with
 // the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair takes
-// about 2400 for 1536: P and dS in turn in the same warps. TMEM (512 columns: S, dP, dV, dK, or two S, dP,
-// dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and 8 heads,
-// causal): 0.83 ms, 830 TFLOP/s of the five products, 1160 of the seven; one of 2048 tokens with 32 and 8
-// heads: 0.125 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
+// about 2000 for 1536: its halves' exponentials in turn, dS beside them. TMEM (512 columns: S, dP, dV, dK, or
+// two S, dP, dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and
+// 8 heads, causal): 0.78 ms, 880 TFLOP/s of the five products, 1230 of the seven; one of 2048 tokens with 32
+// and 8 heads: 0.122 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
 #include <atomic>
 #include <cfloat>
 
@@ -45,7 +45,7 @@ struct BwdLayout {
   static constexpr int NKB = D / ABK;
   static constexpr int TILE_BYTES = NKB * SUB_BYTES;   // 128 rows of one operand
   static constexpr int TILES = 7;                      // key CTA: K, V, 3 Q, 2 dO; query CTA: Q, dO, 3 K, 2 V
-  static constexpr int STAT_BYTES = 5 * 512;           // key CTA: delta with each Q stage, -lse with each dO stage
+  static constexpr int STAT_BYTES = 5 * 512;           // key CTA: -delta with each Q stage, -lse with each dO stage
   static constexpr int BAR_BYTES = 256;
   static constexpr int NEED = TILES * TILE_BYTES + STAT_BYTES + BAR_BYTES;
   static constexpr int SMEM_BYTES = NEED > 116 * 1024 ? NEED : 116 * 1024;   // one CTA per SM: it takes all of TMEM
@@ -59,7 +59,7 @@ struct BwdArgs {
   const int32_t* key_lo;
   const int32_t* key_hi;
   const float* stats;    // [B * Hq][nqt][2][128]: -lse in log2 units (fp16: plus 10; -inf: no key seen, or no such
-                         // row), delta
+                         // row), -delta
   const uint32_t* largest;  // fp16: the bits of the largest |dO_i|^2 and, of visible keys, |v_j|^2
   float* partial;        // [parts][B * Hkv][nkt * 128][2][D] sums of dV and c dK, or null when parts == 1
   uint16_t *dq, *dk, *dv;   // any may be null
@@ -117,13 +117,6 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const i
   }
   return true;
 }
-// s (dP - delta), s being 1 for bf16.
-template <int FMT>
-__device__ __forceinline__ float scaled_less(uint32_t dp, float delta, float s) {
-  const float x = __uint_as_float(dp) - delta;
-  return FMT == 1 ? x : x * s;
-}
-
 // A look at a barrier ahead of time, without a branch: lane 0 polls, the answer is used later by
 // `looked_or_wait`. A poll queues behind the exponentials of both warps of a scheduler (300 cycles and
 // more), which pass meanwhile.
@@ -288,6 +281,19 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const u
 // reads them waits for its end first.
 __device__ __forceinline__ void wait_for_statistics() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// A query CTA's column halves take turns at a tile's exponentials, half 0 first: one has the special-function
+// unit to itself while the other forms dS (both at once: 428 us for dQ of a Llama-3-70B-shaped layer, in turns
+// 376). All eight warps execute every turn, after a timeout too, so that the hardware barriers, which have no
+// time limit, complete. A key CTA's halves do without: what counts there is when the whole of P is written, and
+// one warp per scheduler does not fill the special-function unit (1500 cycles for 1024 of its work).
+constexpr int kTurnBarrier = 1;   // named barriers 1 (half 0's turn) and 2
+__device__ __forceinline__ void turn_wait(int half, int t) {
+  if (half == 1 || t > 0) asm volatile("bar.sync %0, 256;" ::"r"(kTurnBarrier + half) : "memory");
+}
+__device__ __forceinline__ void turn_pass(int half, int t, int n) {
+  if (half == 0 || t + 1 < n) asm volatile("bar.arrive %0, 256;" ::"r"(kTurnBarrier + 1 - half) : "memory");
+}
+
 // What a role that gave up does: the first code stays in the status word.
 __device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int code) {
   atomicCAS(g.status, kErrNone, code);
@@ -383,11 +389,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     query_tile_keys(g, b, qt_own, lo, hi, first, n);
     count = n;
   }
-  // A key CTA's tile t: one Q stage with delta, one dO stage with -lse, as the buffers below are laid out.
+  // A key CTA's tile t: one Q stage with -delta, one dO stage with -lse, as the buffers below are laid out.
   auto load_query_tile = [&](int t, bool q_part, uint32_t phase) {
     const int pair = begin + t, head = (bh_own % g.hkv) * g.group + pair / count, qt = first + pair % count;
     const float* st = g.stats + ((static_cast<int64_t>(b) * g.hq + head) * g.nqt + qt) * 256;
-    float* stat_base = reinterpret_cast<float*>(smem + L::TILES * TILE);   // delta [3][128], -lse [2][128]
+    float* stat_base = reinterpret_cast<float*>(smem + L::TILES * TILE);   // -delta [3][128], -lse [2][128]
     const int s = q_part ? t % 3 : t & 1, bar = (q_part ? 2 : 5) + s;
     armed.arm(bars, bar, phase, TILE + 512);
     load_tile<NKB>(q_part ? &map_q : &map_do, bars + kFull + bar, smem + bar * TILE, qt * AM, head, b);
@@ -436,8 +442,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     uint8_t* sV = smem + TILE;
     uint8_t* sQ = smem + 2 * TILE;        // 3 stages
     uint8_t* sO = smem + 5 * TILE;        // 2 stages
-    float* delta = reinterpret_cast<float*>(smem + L::TILES * TILE);   // [3][128], with Q
-    float* neg_lse = delta + 3 * 128;                                  // [2][128], with dO
+    float* neg_delta = reinterpret_cast<float*>(smem + L::TILES * TILE);   // [3][128], with Q
+    float* neg_lse = neg_delta + 3 * 128;                                  // [2][128], with dO
     const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
 
     if (warp == 0) {
@@ -541,7 +547,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         tc_fence_after();
         const float4* nl = reinterpret_cast<const float4*>(neg_lse + so * 128 + half * 64);
-        const float4* dl = reinterpret_cast<const float4*>(delta + sq * 128 + half * 64);
+        const float4* dl = reinterpret_cast<const float4*>(neg_delta + sq * 128 + half * 64);
         float p[64];
         {
           uint32_t v[64];
@@ -552,10 +558,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
             for (int c = 32 * part; c < 32 * part + 32; c += 4) {
               const float4 m = nl[c >> 2];
-              p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, m.x));
-              p[c + 1] = fast_exp2(fmaf(__uint_as_float(v[c + 1]), g.scale_log2, m.y));
-              p[c + 2] = fast_exp2(fmaf(__uint_as_float(v[c + 2]), g.scale_log2, m.z));
-              p[c + 3] = fast_exp2(fmaf(__uint_as_float(v[c + 3]), g.scale_log2, m.w));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[c + e] = __uint_as_float(v[c + e]);
+              fma_pair(p[c], p[c + 1], g.scale_log2, m.x, m.y);
+              fma_pair(p[c + 2], p[c + 3], g.scale_log2, m.z, m.w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[c + e] = fast_exp2(p[c + e]);
             }
             if (!all_seen) {
 #pragma unroll
@@ -580,11 +588,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 m = dl[(ch * 32 + c) >> 2];
-            float* pp = p + ch * 32 + c;
-            pp[0] *= scaled_less<FMT>(v[c], m.x, two.ds);
-            pp[1] *= scaled_less<FMT>(v[c + 1], m.y, two.ds);
-            pp[2] *= scaled_less<FMT>(v[c + 2], m.z, two.ds);
-            pp[3] *= scaled_less<FMT>(v[c + 3], m.w, two.ds);
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[c + e]);
+            add_pair(x[0], x[1], m.x, m.y);
+            add_pair(x[2], x[3], m.z, m.w);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              if (FMT == 0) mul_pair(x[e], x[e + 1], two.ds, two.ds);
+              mul_pair(p[ch * 32 + c + e], p[ch * 32 + c + e + 1], x[e], x[e + 1]);
+            }
           }
         }
         if (!all_seen) {   // a masked pair's dP may be anything (a key's V outside its range)
@@ -713,8 +726,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const float* st = g.stats + (bh * g.nqt + qt) * 256;
       wait_for_statistics();
       const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
-      const float nl = n > 0 ? st[r] : 0.0f, delta = n > 0 ? st[128 + r] : 0.0f;
-      const float delta_ds = -delta * two.ds;
+      const float nl = n > 0 ? st[r] : 0.0f, nd = n > 0 ? st[128 + r] * two.ds : 0.0f;
       int64_t end = hi;                                      // visible keys of this row: [lo, end)
       if (g.causal && row + g.shift + 1 < end) end = row + g.shift + 1;
       if (!row_in) end = lo;
@@ -725,6 +737,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
       }
       uint32_t s_here = 0;   // a look at the next S
+      int turns = 0;         // turns taken and passed on
       for (int t = 0; t < n && ok; ++t) {
         const int64_t key0 = static_cast<int64_t>(first + t) * AN;
         const int64_t a0 = lo - key0 - 64 * half, a1 = end - key0 - 64 * half;
@@ -739,12 +752,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         {
           uint32_t v[64];
           tmem_ld64(my_s, v);
+          turn_wait(half, t);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
-          dp_here = look(bars + kDp, t & 1);
-#pragma unroll
-          for (int c = 32; c < 64; ++c) p[c] = fast_exp2(fmaf(__uint_as_float(v[c]), g.scale_log2, nl));
+          for (int c = 0; c < 64; c += 2) {
+            if (c == 32) dp_here = look(bars + kDp, t & 1);
+            p[c] = __uint_as_float(v[c]);
+            p[c + 1] = __uint_as_float(v[c + 1]);
+            fma_pair(p[c], p[c + 1], g.scale_log2, nl, nl);
+            p[c] = fast_exp2(p[c]);
+            p[c + 1] = fast_exp2(p[c + 1]);
+          }
         }
+        turn_pass(half, t, n);
+        turns = t + 1;
         if (!looked_or_wait(dp_here, bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         {
@@ -755,8 +775,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (lane == 0) mbar_arrive(bars + kP);   // dP(t) read: the next one may be formed
           s_here = look(bars + kS + ((t + 1) & 1), ((t + 1) >> 1) & 1);
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            p[c] *= FMT == 1 ? __uint_as_float(v[c]) - delta : fmaf(__uint_as_float(v[c]), two.ds, delta_ds);
+          for (int c = 0; c < 64; c += 2) {
+            float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
+            if (FMT == 1) add_pair(x0, x1, nd, nd);
+            else fma_pair(x0, x1, two.ds, nd, nd);
+            mul_pair(p[c], p[c + 1], x0, x1);
+          }
         }
         if (!all_seen) {   // a masked pair's dP may be anything (V of a key outside the range)
 #pragma unroll
@@ -779,6 +803,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kDs + (t & 1));
+      }
+      for (; turns < n; ++turns) {   // this warp gave up: its turns pass all the same
+        turn_wait(half, turns);
+        turn_pass(half, turns, n);
       }
       if (ok && n > 0) {
         ok = warp_wait(bars + kDone, 0, abort_flag);
@@ -857,7 +885,7 @@ struct Rows16 {   // a [B][H][S][D] operand of 16-bit elements
 };
 
 // Per query row: -lse in log2 units (with the power of two that P carries; -inf for a row that sees no
-// key, so that its probabilities are 0) and delta = dO . O, in tiles of 128 rows padded with such rows: one
+// key, so that its probabilities are 0) and -delta = -dO . O, in tiles of 128 rows padded with such rows: one
 // block per tile, 16 lanes per row (8 elements each), four rows per lane with their loads in flight
 // together. For fp16 also the largest |dO_i|^2 and, in the blocks behind the query tiles', the largest
 // |v_j|^2 of the keys inside their range.
@@ -924,7 +952,7 @@ attn_bwd_stats_kernel(Rows16 o, Rows16 d, Rows16 v, const float* lse, float* sta
     if (FMT == 0) square = larger(square, sum16(here && in ? s : 0.0f));
     if (l == 0) {
       tile[row] = w[r] == -INFINITY ? -INFINITY : fmaf(-w[r], kLog2e, FMT == 0 ? 10.0f : 0.0f);   // fp16: 2^10 P
-      tile[128 + row] = sum;
+      tile[128 + row] = -sum;
     }
   }
   if (FMT == 0) block_largest(square, largest);

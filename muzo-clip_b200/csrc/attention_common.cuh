@@ -19,22 +19,31 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 
 // Two fp32 values in one instruction of the FMA pipe, each rounded once as its scalar form is:
-// x = x * a + b, and x += y.
-__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a, float b) {
+// x = x * a + (b0, b1), x += y, x *= y.
+__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a, float b0, float b1) {
   asm("{\n\t.reg .b64 x, a, b;\n\t"
       "mov.b64 x, {%0, %1};\n\t"
       "mov.b64 a, {%2, %2};\n\t"
-      "mov.b64 b, {%3, %3};\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
       "fma.rn.f32x2 x, x, a, b;\n\t"
       "mov.b64 {%0, %1}, x;\n\t}"
       : "+f"(x0), "+f"(x1)
-      : "f"(a), "f"(b));
+      : "f"(a), "f"(b0), "f"(b1));
 }
 __device__ __forceinline__ void add_pair(float& x0, float& x1, float y0, float y1) {
   asm("{\n\t.reg .b64 x, y;\n\t"
       "mov.b64 x, {%0, %1};\n\t"
       "mov.b64 y, {%2, %3};\n\t"
       "add.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ void mul_pair(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\t"
       "mov.b64 {%0, %1}, x;\n\t}"
       : "+f"(x0), "+f"(x1)
       : "f"(y0), "f"(y1));
