@@ -19,8 +19,8 @@
 //
 // What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1100 cycles, of
 // which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2700 cycles with
-// the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair takes
-// about 2000 for 1536: its halves' exponentials in turn, dS beside them. TMEM (512 columns: S, dP, dV, dK, or
+// the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair has 1536:
+// its halves' exponentials in turn, dS beside them, 1.5 us of an SM. TMEM (512 columns: S, dP, dV, dK, or
 // two S, dP, dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and
 // 8 heads, causal): 0.78 ms, 880 TFLOP/s of the five products, 1230 of the seven; one of 2048 tokens with 32
 // and 8 heads: 0.122 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
@@ -288,9 +288,11 @@ __device__ __forceinline__ void wait_for_statistics() { asm volatile("griddepcon
 // one warp per scheduler does not fill the special-function unit (1500 cycles for 1024 of its work).
 constexpr int kTurnBarrier = 1;   // named barriers 1 (half 0's turn) and 2
 __device__ __forceinline__ void turn_wait(int half, int t) {
+  __syncwarp();   // the barrier instructions want their warp converged
   if (half == 1 || t > 0) asm volatile("bar.sync %0, 256;" ::"r"(kTurnBarrier + half) : "memory");
 }
 __device__ __forceinline__ void turn_pass(int half, int t, int n) {
+  __syncwarp();
   if (half == 0 || t + 1 < n) asm volatile("bar.arrive %0, 256;" ::"r"(kTurnBarrier + 1 - half) : "memory");
 }
 
