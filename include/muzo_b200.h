@@ -320,10 +320,10 @@ int muzo_max_merge(float* running, const float* fresh, const int32_t* d_valid, i
  * eager capture of qk_clip.py:173-196 taken from the attention the forward computes anyway, so
  * Q K^T is formed once (no counterpart in the reference, whose capture needs eager attention).
  * Q [B, Hq, Sq, D], K and V [B, Hkv, Sk, D] (element strides, D contiguous, GQA kv head
- * h / (Hq / Hkv)), bf16 or fp16, D = 64 or 128; out[b, h, i, :] at o_stride_b * b + o_stride_h
+ * h / (Hq / Hkv)), bf16 or fp16, D a multiple of 8 up to 128; out[b, h, i, :] at o_stride_b * b + o_stride_h
  * * h + o_stride_s * i (for transformers' [B, Sq, Hq, D] output: Sq*Hq*D, D, Hq*D) receives
  * softmax(scale * Q K^T) V over the visible keys (fp32 accumulation, P rounded to the input
- * dtype as flash attention does), zeros for a row without a visible key. Key j is visible to
+ * dtype, the products' operand type), zeros for a row without a visible key. Key j is visible to
  * query i of batch b when d_key_lo[b] <= j < d_key_hi[b] (device int32 per batch; NULL: 0 and
  * Sk) and, when causal, j <= i + Sk - Sq. With smax non-NULL, smax[h] (float[Hq], overwritten)
  * = dtype(dtype(max over the visible logits of q . k) * scale) and *d_valid = 0 when a visible
@@ -343,8 +343,8 @@ int muzo_attention_max(const void* q, const void* k, const void* v, void* out, i
 /* muzo_attention_max that also keeps, when lse is non-NULL, the natural logarithm of each row's sum
  * of exp(scale * logit) over its visible keys, lse[b][h][i] (float[B * Hq * Sq], -inf for a row
  * that sees none): the statistic muzo_attention_backward recomputes the probabilities from. The
- * scale must then be positive. D may be any multiple of 8 up to 128 (here and in
- * muzo_attention_max); Sk = 0 is allowed (K and V may then be NULL) and writes zeros. */
+ * scale must then be positive. Sk = 0 is allowed, here and in muzo_attention_max (K and V may then
+ * be NULL), and writes zeros. */
 int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* out, float* lse, int dtype,
                            int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
                            int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
