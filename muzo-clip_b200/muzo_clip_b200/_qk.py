@@ -276,7 +276,7 @@ def _probe_attention(module, query, key, value, attention_mask, scaling=None, dr
         ranges = None if mask is None else mask_key_ranges(mask, query.shape[0], sq, key.shape[2])
         name = ctrl.module_name(module)
         if name is not None and (mask is None or ranges is not None) and \
-                fused_attention_eligible(query, key, value, dropout):
+                fused_attention_eligible(query, key, value, dropout) and scaling > 0.0:
             if ranges is None:
                 causal, lo, hi = bool(getattr(module, "is_causal", True)) and sq > 1, None, None
             else:

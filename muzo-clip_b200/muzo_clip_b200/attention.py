@@ -55,7 +55,8 @@ def attention_max(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, s
 
     Differentiable once in query, key and value (the maxima are not): the products of the backward
     pass take the probabilities and their gradients in the inputs' type, as the forward does, and
-    sum in fp32."""
+    sum in fp32. A backward pass can be captured into a CUDA graph while no graph of the same leaves
+    that was built on another stream is alive (torch ends such a capture with an error)."""
     return _native.attention(query, key, value, scaling, causal, key_lo, key_hi, record)
 
 

@@ -88,6 +88,41 @@ def test_the_fused_kernel_runs_and_falls_back(device, monkeypatch):
     assert len(calls) == 4
 
 
+@pytest.mark.parametrize("scaling", [-0.5, 0.0])
+def test_capture_with_a_scale_the_kernel_refuses(device, monkeypatch, scaling):
+    """MUZO_FUSED_ATTENTION=1, a scale that is not positive: the capture runs on SDPA, as without it."""
+    from muzo_clip_b200 import _qk, attention_max
+
+    class Recorder:
+        kept = []
+
+        def module_name(self, module):
+            return "layer"
+
+        def record_qk(self, module, query, key, scale, causal, mask):
+            self.kept.append((scale, causal))
+
+        def record_max(self, name, smax, valid):
+            raise AssertionError("the fused kernel took a scale that it refuses")
+
+    monkeypatch.setenv("MUZO_FUSED_ATTENTION", "1")
+    gen = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn((2, 4, 33, 64), generator=gen).to(device, torch.bfloat16) for _ in range(3))
+    module = torch.nn.Module()
+    module.is_causal = True
+    recorder = Recorder()
+    token = _qk._ACTIVE.set(recorder)
+    try:
+        with torch.no_grad():
+            out, _ = _qk._probe_attention(module, q, k, v, None, scaling=scaling)
+    finally:
+        _qk._ACTIVE.reset(token)
+    ref = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scaling).transpose(1, 2)
+    assert torch.equal(out, ref) and recorder.kept == [(scaling, True)]
+    with pytest.raises(ValueError, match="scaling must be positive"):
+        attention_max(q, k, v, scaling)
+
+
 def test_step_with_clipping_and_qk_clip(device):
     """One gradient step as a user writes it: forward under capture, backward, clip, update; then
     QK-Clip on the captured maxima, which are the eager ones; the zeroth-order projection still runs
