@@ -19,11 +19,11 @@
 //
 // What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1100 cycles, of
 // which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2700 cycles with
-// the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair has 1536:
-// its halves' exponentials in turn, dS beside them, 1.5 us of an SM. TMEM (512 columns: S, dP, dV, dK, or
+// the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair takes
+// about 2400 for 1536: P and dS in turn in the same warps. TMEM (512 columns: S, dP, dV, dK, or
 // two S, dP, dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and
-// 8 heads, causal): 0.78 ms, 880 TFLOP/s of the five products, 1230 of the seven; one of 2048 tokens with 32
-// and 8 heads: 0.122 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
+// 8 heads, causal): 0.79 ms, 870 TFLOP/s of the five products, 1220 of the seven; one of 2048 tokens with 32
+// and 8 heads: 0.121 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
 #include <atomic>
 #include <cfloat>
 
@@ -280,21 +280,6 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const u
 // The kernel may start while the one that writes the statistics still runs (programmatic launch): who
 // reads them waits for its end first.
 __device__ __forceinline__ void wait_for_statistics() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// A query CTA's column halves take turns at a tile's exponentials, half 0 first: one has the special-function
-// unit to itself while the other forms dS (both at once: 428 us for dQ of a Llama-3-70B-shaped layer, in turns
-// 376). All eight warps execute every turn, after a timeout too, so that the hardware barriers, which have no
-// time limit, complete. A key CTA's halves do without: what counts there is when the whole of P is written, and
-// one warp per scheduler does not fill the special-function unit (1500 cycles for 1024 of its work).
-constexpr int kTurnBarrier = 1;   // named barriers 1 (half 0's turn) and 2
-__device__ __forceinline__ void turn_wait(int half, int t) {
-  __syncwarp();   // the barrier instructions want their warp converged
-  if (half == 1 || t > 0) asm volatile("bar.sync %0, 256;" ::"r"(kTurnBarrier + half) : "memory");
-}
-__device__ __forceinline__ void turn_pass(int half, int t, int n) {
-  __syncwarp();
-  if (half == 0 || t + 1 < n) asm volatile("bar.arrive %0, 256;" ::"r"(kTurnBarrier + 1 - half) : "memory");
-}
 
 // What a role that gave up does: the first code stays in the status word.
 __device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int code) {
@@ -739,7 +724,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
       }
       uint32_t s_here = 0;   // a look at the next S
-      int turns = 0;         // turns taken and passed on
       for (int t = 0; t < n && ok; ++t) {
         const int64_t key0 = static_cast<int64_t>(first + t) * AN;
         const int64_t a0 = lo - key0 - 64 * half, a1 = end - key0 - 64 * half;
@@ -754,7 +738,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         {
           uint32_t v[64];
           tmem_ld64(my_s, v);
-          turn_wait(half, t);
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
             if (c == 32) dp_here = look(bars + kDp, t & 1);
@@ -765,8 +748,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             p[c + 1] = fast_exp2(p[c + 1]);
           }
         }
-        turn_pass(half, t, n);
-        turns = t + 1;
         if (!looked_or_wait(dp_here, bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         {
@@ -805,10 +786,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kDs + (t & 1));
-      }
-      for (; turns < n; ++turns) {   // this warp gave up: its turns pass all the same
-        turn_wait(half, turns);
-        turn_pass(half, turns, n);
       }
       if (ok && n > 0) {
         ok = warp_wait(bars + kDone, 0, abort_flag);
