@@ -299,8 +299,8 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             umma_f16(tmem_base + s * AN, make_sdesc(sq_ + kb * SUB_BYTES + k * 32, 16, 1024),
                      make_sdesc(sk_ + kb * SUB_BYTES + k * 32, 16, 1024), idesc_s, (kb > 0 || k > 0) ? 1u : 0u);
         umma_commit(s_full + s);
-        umma_commit(k_empty + stage);
-        return true;
+        if (j + K_STAGES < ntiles) umma_commit(k_empty + stage);   // nothing is committed that nobody waits for:
+        return true;                                               // it might arrive after the CTA's end
       };
       auto issue_pv = [&](int j) -> bool {
         const int stage = j % VS;
@@ -318,7 +318,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             umma_f16(tmem_o + s * D, make_sdesc(sp + kc * SUB_BYTES + k * 32, 16, 1024),
                      make_sdesc(sv + kc * NKB * BOX_BYTES + k * (16 * 128), BOX_BYTES, 1024), idesc_pv,
                      (j > 0 || kc > 0 || k > 0) ? 1u : 0u);
-        umma_commit(v_empty + stage);
+        if (j + VS < ntiles) umma_commit(v_empty + stage);
         umma_commit(o_done + s);        // P buffer of the stream free, O_s holds its tiles up to j
         return true;
       };
@@ -385,6 +385,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // run. 128 of the thread's 168 registers hold the row (both passes reading TMEM instead:
       // 314 us against 286 for a Llama-3-70B-shaped layer).
       uint32_t v[AN];
+      __syncwarp();
       tmem_ld128(s_cols, v);
       tc_fence_before();
       __syncwarp();
@@ -433,11 +434,13 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {   // 16 at a time: S holds most of the registers
           uint32_t o[16];
+          __syncwarp();
           tmem_ld16(o_cols + c * 16, o);
           if (rescale) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
           }
+          __syncwarp();
           tmem_st16(o_cols + c * 16, o);
         }
       }
@@ -512,6 +515,7 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
         if (n_mine > 0) {
+          __syncwarp();
           tmem_ld32(o_cols + c * 32, v);
         } else {
 #pragma unroll

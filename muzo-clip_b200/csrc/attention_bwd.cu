@@ -22,8 +22,8 @@
 // the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair takes
 // about 2400 for 1536: P and dS in turn in the same warps. TMEM (512 columns: S, dP, dV, dK, or
 // two S, dP, dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and
-// 8 heads, causal): 0.79 ms, 870 TFLOP/s of the five products, 1220 of the seven; one of 2048 tokens with 32
-// and 8 heads: 0.121 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
+// 8 heads, causal): 0.80 ms, 860 TFLOP/s of the five products, 1200 of the seven; one of 2048 tokens with 32
+// and 8 heads: 0.123 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
 #include <atomic>
 #include <cfloat>
 
@@ -136,6 +136,7 @@ __device__ __forceinline__ uint32_t look(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const int* abort_flag) {
   bool ready = true;
   if ((threadIdx.x & 31) == 0) ready = wait_one(bar, parity, abort_flag);
+  __syncwarp();
   return __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
 }
 
@@ -216,7 +217,9 @@ __device__ __forceinline__ void scale_row(const uint32_t (&v)[32], float f, uint
                       __float_as_uint(__uint_as_float(v[4 * c + 2]) * f), __float_as_uint(__uint_as_float(v[4 * c + 3]) * f));
 }
 
-// Barriers of both kinds of CTA.
+// Barriers of both kinds of CTA. Every arrival that an issuer commits to is waited for before the CTA ends (a
+// stage that no later tile takes is not released): two commits behind the same product have no stated order,
+// and one that came after the other's waiters had left would write to shared memory that is another's.
 enum : int {
   kFull = 0,        // key CTA: K, V, Q[3], dO[2]; query CTA: Q, dO, K[3], V[2]
   kEmpty = 7,       // key CTA: Q[3], dO[2] (at 2 and 5); query CTA: K[3], V[2] (at 2 and 5)
@@ -281,6 +284,9 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, const u
 // reads them waits for its end first.
 __device__ __forceinline__ void wait_for_statistics() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// TMEM loads and stores are instructions of a whole converged warp: each stands behind a __syncwarp, since a
+// lane may have polled or arrived alone before it.
+
 // What a role that gave up does: the first code stays in the status word.
 __device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int code) {
   atomicCAS(g.status, kErrNone, code);
@@ -333,16 +339,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int stall = *reinterpret_cast<volatile int*>(g.status + 1);
   const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
 
-  if (warp == 0) {
+  if (threadIdx.x == 0) {
+    // One thread initialises every barrier, and no load is issued before the CTA's barrier below. (Initialised by a
+    // lane each, and used by the first loads behind a __syncwarp, they began 2 to 4 us earlier, but nothing ordered
+    // the other lanes' initialisations before the loads' arrivals: a launch in some ten thousand faulted.)
     // arrivals: the eight probability warps on kP and kDs, the warp that waits for a key CTA's loads on its second
     // kP, a query CTA's two issuers on kDone
-    static_assert(kBars <= 32, "one lane per barrier");
-    const int i = lane;
-    if (i < kBars)
+    for (int i = 0; i < kBars; ++i)
       mbar_init(bars + i, i == kP + 1 ? 9 : (i >= kP && i < kDone ? 8 : (i == kDone && !key_cta ? 2 : 1)));
-    if (lane == 0) *abort_flag = 0;
+    *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
@@ -350,7 +356,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // The CTA's work, and the producer's first loads: they run while the others still wait for TMEM.
+  // The CTA's work
   Armed armed;
   int kt = 0, qt_own = 0, b, bh_own, first, count, begin = 0, n;
   int64_t lo, hi;
@@ -398,6 +404,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     armed.arm(bars, bar, 0, TILE);
     load_tile<NKB>(map, bars + kFull + bar, smem + bar * TILE, row, head, b);
   };
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // All 512 columns: they begin at 0. (An address that says otherwise is reported, and the CTA does nothing.)
+  constexpr uint32_t tmem = 0;
+  const bool tmem_ok = *reinterpret_cast<volatile uint32_t*>(tmem_holder) == tmem;
+  if (!tmem_ok) {
+    give_up(g, abort_flag, kErrTimeoutMma);
+    n = 0;
+  }
   if (threadIdx.x == 0 && n > 0) {
     if (key_cta) {
       load_own(&map_k, 0, kt * AN, bh_own % g.hkv);
@@ -411,10 +427,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       load_key_tile(0, false, 0);
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
   constexpr uint32_t idesc_s = make_idesc_fmt(128, 128, false, false, FMT);   // S, dP: both operands K-major
   constexpr uint32_t idesc_g = make_idesc_fmt(128, D, false, true, FMT);      // gradients: B MN-major
   const int quarter = warp & 3, half = (warp - 4) >> 2;
@@ -474,14 +486,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, t > 0, 64, 0);
           if (!ready(kP + 1, t & 1)) { ok = false; break; }
           mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, true, 64, 1);
-          umma_commit(bars + kEmpty + 5 + so);
+          if (t + 2 < n) umma_commit(bars + kEmpty + 5 + so);
           if (t + 1 < n) {
             mma_ss<NKB>(t_s, sK, sQ + ((t + 1) % 3) * TILE, idesc_s);
             umma_commit(bars + kS);
           }
           if (!ready(kDs, t & 1)) { ok = false; break; }
           mma_ts(t_dk, t_dp, sQ + (t % 3) * TILE, idesc_g, t > 0, 64);
-          umma_commit(bars + kEmpty + 2 + t % 3);
+          if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
           if (t + 1 < n) {
             mma_ss<NKB>(t_dp, sV, sO + (so ^ 1) * TILE, idesc_s);
             umma_commit(bars + kDp);
@@ -538,6 +550,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         float p[64];
         {
           uint32_t v[64];
+          __syncwarp();
           tmem_ld64(t_s + lane_addr + half * 64, v);
           // P by halves, so that dV begins while the second half's exponentials run
 #pragma unroll
@@ -559,6 +572,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             uint32_t w[16];
 #pragma unroll
             for (int c = 0; c < 16; ++c) w[c] = pack16<FMT>(p[32 * part + 2 * c], p[32 * part + 2 * c + 1]);
+            __syncwarp();
             tmem_st16(t_s + lane_addr + half * 64 + 16 * part, w);
             tc_fence_before();
             __syncwarp();
@@ -571,6 +585,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
           uint32_t v[32];
+          __syncwarp();
           tmem_ld32(t_dp + lane_addr + half * 64 + ch * 32, v);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
@@ -593,6 +608,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
 #pragma unroll
         for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
+        __syncwarp();
         tmem_st32(t_dp + lane_addr + half * 64, w);
         tc_fence_before();
         __syncwarp();
@@ -617,6 +633,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           for (int c = 0; c < D / 32; ++c) {
             uint32_t v[32];
             uint4 w[8];
+            __syncwarp();
             tmem_ld32(acc + c * 32, v);
             scale_row(v, f, w);
             store_rows(stage, w, sum + c * 128, 2 * D * 4, 32, 8);
@@ -631,6 +648,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               uint4 w[8];
               if (n > 0) {
                 uint32_t v[64];
+                __syncwarp();
                 tmem_ld64(acc + c * 64, v);
                 pack_row<FMT>(v, f, w);
               } else {
@@ -691,7 +709,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (t + 2 < n && !ready(kFull + 2 + (t + 2) % 3, ((t + 2) / 3) & 1)) { ok = false; break; }
             if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
             mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0, 64);
-            umma_commit(bars + kEmpty + 2 + t % 3);
+            if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
             if (t + 2 < n) issue_s(t + 2);
           }
         } else {
@@ -700,7 +718,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1) || (t > 0 && !ready(kP, (t - 1) & 1))) { ok = false; break; }
             mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
             umma_commit(bars + kDp);
-            umma_commit(bars + kEmpty + 5 + (t & 1));
+            if (t + 2 < n) umma_commit(bars + kEmpty + 5 + (t & 1));
           }
         }
         if (ok) umma_commit(bars + kDone);
@@ -737,6 +755,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         uint32_t dp_here;
         {
           uint32_t v[64];
+          __syncwarp();
           tmem_ld64(my_s, v);
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
@@ -752,6 +771,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tc_fence_after();
         {
           uint32_t v[64];
+          __syncwarp();
           tmem_ld64(t_dp + lane_addr + half * 64, v);
           tc_fence_before();
           __syncwarp();
@@ -772,6 +792,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         uint32_t w[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
+        __syncwarp();
         tmem_st32(my_s, w);
         // keys outside [lo, hi) beside visible ones: their dS is 0, but 0 times a non-finite key would
         // still reach dQ, so their K rows (S(t) has read them) are cleared
@@ -801,6 +822,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           uint4 w[8];
           if (n > 0) {
             uint32_t v[64];
+            __syncwarp();
             tmem_ld64(t_dq + lane_addr + col0, v);
             pack_row<FMT>(v, g.scale * two.dqk, w);
           } else {
@@ -828,7 +850,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   }
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(B_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*reinterpret_cast<volatile uint32_t*>(tmem_holder)), "r"(B_TMEM_COLS) : "memory");
   }
 }
 
