@@ -554,6 +554,51 @@ print("the same")
     assert done.returncode == 0 and "the same" in done.stdout, done.stdout + done.stderr
 
 
+FRESH = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from muzo_clip_b200 import _lib
+gen = torch.Generator(device="cuda").manual_seed(5)
+q, k, v, dout = (torch.randn((1, 2048, h, 128), generator=gen, device="cuda").bfloat16() for h in (32, 8, 8, 32))
+q, k, v = (x.transpose(1, 2) for x in (q, k, v))
+native = _lib.native
+out, lse, _, _ = native.attention_forward(q, k, v, None, True, None, None, False, True)
+def grads(*wanted):
+    return native.attention_backward(dout, q, k, v, out, lse, None, True, None, None, wanted)
+first = grads(True, True, True)
+for wanted in ((True, True, True), (True, False, False), (False, True, True)):
+    torch.cuda.empty_cache()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = [grads(*wanted) for _ in range(5)]
+    for _ in range(3):
+        graph.replay()
+    again = grads(*wanted)
+    torch.cuda.synchronize()
+    split = wanted != (True, True, True)   # without dQ the key tiles may be divided: another order of their sums
+    for got in results + [again]:
+        for name, a, b in zip(("dq", "dk", "dv"), got, again):
+            assert a is None and b is None or torch.equal(a, b), name
+        for name, a, b in zip(("dq", "dk", "dv"), got, first):
+            assert a is None or (split and name != "dq") or torch.equal(a, b), name
+    del graph, results, again
+print("same")
+"""
+
+
+@pytest.mark.parametrize("process", range(3))
+def test_first_launches_of_fresh_processes(device, process):
+    """The first launches of a process, eager and replayed, behind other kernels' data in shared memory and with memory
+    mapped and released in between: both kinds of CTA together, and each alone, give the same bits every time."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    done = subprocess.run([sys.executable, "-c", FRESH, str(ROOT / "muzo-clip_b200")], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "same", done.stderr[-2000:]
+
+
 def test_refusals(device):
     from muzo_clip_b200 import attention_max, attention_max_backward
 
