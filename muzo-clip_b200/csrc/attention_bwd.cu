@@ -427,6 +427,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       load_key_tile(0, false, 0);
     }
   }
+  if (warp == 3) wait_for_statistics();   // in CTAs that read none too: this launch ends after the one it may overlap
   constexpr uint32_t idesc_s = make_idesc_fmt(128, 128, false, false, FMT);   // S, dP: both operands K-major
   constexpr uint32_t idesc_g = make_idesc_fmt(128, D, false, true, FMT);      // gradients: B MN-major
   const int quarter = warp & 3, half = (warp - 4) >> 2;
