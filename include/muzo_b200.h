@@ -357,7 +357,8 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
 /* Gradients of that attention (no counterpart in the reference, which trains without gradients):
  * with P = exp(scale * Q K^T - lse) over the visible pairs, dP = dO V^T, delta = rowsum(dO * O) and
  * dS = P * (dP - delta):  dV = P^T dO, dK = scale * dS^T Q, dQ = scale * dS K, dK and dV summed over
- * the Hq / Hkv query heads of a key head. P and dS enter the products in the input type, sums are
+ * the Hq / Hkv query heads of a key head. A row that sees no key has no gradient and gives none, whatever
+ * its Q and dO hold. P and dS enter the products in the input type, sums are
  * fp32. Nothing is added atomically: equal calls give equal bits. Any of dq, dk, dv may be NULL
  * (dq alone, or dk and dv, skip the other's work). `strides` (host memory, 24 entries): the element
  * strides (batch, head, sequence) of q, k, v, out, dout, dq, dk, dv, all multiples of 8 and, for the

@@ -60,7 +60,7 @@ struct BwdArgs {
   const int32_t* key_hi;
   const float* stats;    // [B * Hq][nqt][2][128]: -lse in log2 units (fp16: plus 10; -inf: no key seen, or no such
                          // row), -delta
-  const uint32_t* largest;  // fp16: the bits of the largest |dO_i|^2 and, of visible keys, |v_j|^2
+  const uint32_t* largest;  // fp16: the bits of the largest |dO_i|^2 of rows that see a key and, of visible keys, |v_j|^2
   float* partial;        // [parts][B * Hkv][nkt * 128][2][D] sums of dV and c dK, or null when parts == 1
   uint16_t *dq, *dk, *dv;   // any may be null
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
@@ -523,6 +523,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
       const int64_t key = static_cast<int64_t>(kt) * AN + r;
       const bool key_seen = key >= lo && key < hi;
+      const int64_t blind = g.causal ? lo - g.shift : 0;   // rows in front of the first that sees a key
+      const int blind_rows = blind > 0 ? static_cast<int>(blind % AM) : 0;
+      const int blind_tile = blind_rows > 0 ? static_cast<int>(blind / AM) : -1;
       bool ok = true;
       if (stall == kErrTimeoutEpilogue) {
         bool waited = true;
@@ -546,6 +549,20 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           break;
         }
         tc_fence_after();
+        // The first rows of a head's first tile may see no key (left padding under causality, more queries than
+        // keys). Their P and dS are 0, but 0 times a non-finite dO or Q would still reach dV and dK, so those rows
+        // are cleared: dO's once dP(t) has read them, Q's (S(t) has read them) now.
+        if (qt == blind_tile) {
+          if (half == 0 && !warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
+          if (r < blind_rows) {
+            uint8_t* row = (half == 0 ? sO + so * TILE : sQ + sq * TILE) + r * 128;
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(row + kb * SUB_BYTES + 16 * e) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
         const float4* nl = reinterpret_cast<const float4*>(neg_lse + so * 128 + half * 64);
         const float4* dl = reinterpret_cast<const float4*>(neg_delta + sq * 128 + half * 64);
         float p[64];
@@ -889,8 +906,8 @@ struct Rows16 {   // a [B][H][S][D] operand of 16-bit elements
 // Per query row: -lse in log2 units (with the power of two that P carries; -inf for a row that sees no
 // key, so that its probabilities are 0) and -delta = -dO . O, in tiles of 128 rows padded with such rows: one
 // block per tile, 16 lanes per row (8 elements each), four rows per lane with their loads in flight
-// together. For fp16 also the largest |dO_i|^2 and, in the blocks behind the query tiles', the largest
-// |v_j|^2 of the keys inside their range.
+// together. For fp16 also the largest |dO_i|^2 of the rows that see a key and, in the blocks behind the query
+// tiles', the largest |v_j|^2 of the keys inside their range.
 template <int FMT>
 __global__ void __launch_bounds__(kStatThreads, 2)
 attn_bwd_stats_kernel(Rows16 o, Rows16 d, Rows16 v, const float* lse, float* stats, uint32_t* largest, int hq, int64_t sq,
@@ -951,7 +968,10 @@ attn_bwd_stats_kernel(Rows16 o, Rows16 d, Rows16 v, const float* lse, float* sta
       if (FMT == 0) s = fmaf(y[r][e], y[r][e], s);
     }
     sum = sum16(here && in ? sum : 0.0f);
-    if (FMT == 0) square = larger(square, sum16(here && in ? s : 0.0f));
+    if (FMT == 0) {   // a row that sees no key may hold anything
+      const bool seen = __shfl_sync(0xffffffffu, w[r], 0, 16) != -INFINITY;
+      square = larger(square, sum16(here && in && seen ? s : 0.0f));
+    }
     if (l == 0) {
       tile[row] = w[r] == -INFINITY ? -INFINITY : fmaf(-w[r], kLog2e, FMT == 0 ? 10.0f : 0.0f);   // fp16: 2^10 P
       tile[128 + row] = -sum;
