@@ -14,8 +14,10 @@
 //               S = Q K^T, dP = dO V^T, dQ += dS K.
 // Forming S and dP twice costs 7 products instead of 5, and saves the fp32 dQ that would have to be
 // added up in memory in a fixed order. P and dS are the first operands of their products straight from
-// TMEM, over the columns of the S and dP they came from, so shared memory holds operand tiles only (three
-// Q and two dO stages, or three K and two V stages, beside the resident pair).
+// TMEM (over the columns of the S and dP they came from, where there is no room beside them), so shared memory
+// holds operand tiles only (three Q and two dO stages, or three K and two V stages, beside the resident pair).
+// Columns that a product reads are taken by the next S or dP once a commit has told that it has run: only MMAs
+// of the same accumulator and shape are promised to run in the order they are issued.
 //
 // What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1100 cycles, of
 // which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2700 cycles with
@@ -231,7 +233,8 @@ enum : int {
   kDone = 21,
   kDrain = 22,      // two: one per issuer
   kStall = 24,
-  kBars = 25
+  kOrder = 25,      // two: a product has read its A operand from TMEM, and the next S or dP may take the columns
+  kBars = 27
 };
 
 // Loads issued by the producer thread: which full barriers are armed, and with which parity.
@@ -444,7 +447,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     uint8_t* sO = smem + 5 * TILE;        // 2 stages
     float* neg_delta = reinterpret_cast<float*>(smem + L::TILES * TILE);   // [3][128], with Q
     float* neg_lse = neg_delta + 3 * 128;                                  // [2][128], with dO
-    const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+    // Tiles of 64 columns leave room for P and dS beside S and dP. Those of 128 do not: P and dS lie over the first
+    // halves of the columns that their warps read, and the next S and dP, which overwrite them, have to wait until
+    // dV and dK have read them: MMAs of different accumulators or shapes have no promised order.
+    constexpr bool kOwn = D == 64;
+    constexpr int kSecond = kOwn ? 32 : 64;   // columns from the first 64 K rows to the others
+    const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = t_dv + D;
+    const uint32_t t_p = kOwn ? tmem + 384 : t_s, t_ds = kOwn ? tmem + 448 : t_dp;
 
     if (warp == 0) {
       if (lane == 0 && n > 0) {
@@ -468,6 +477,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           tc_fence_after();
           return true;
         };
+        auto read_by_now = [&](int which, int t) -> bool {   // what has been issued has run
+          umma_commit(bars + kOrder + which);
+          return ready(kOrder + which, t & 1);
+        };
         bool ok = stall != kErrTimeoutMma || mbar_wait(bars + kStall, 0, kStallLimitCycles);
         ok = ok && ready(kFull, 0) && ready(kFull + 2, 0);
         if (ok) {
@@ -481,21 +494,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         for (int t = 0; t < n && ok; ++t) {
           const int so = t & 1;
-          // P(t) written over S(t), the next Q and dO loaded (warp 2 arrives for them): dV, then the next S
-          // over P(t) (MMAs run in the order they are issued)
+          // P(t) written, S(t) read, the next Q and dO loaded (warp 2 arrives for them): dV, then the next S
           if (!ready(kP, t & 1)) { ok = false; break; }
-          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, t > 0, 64, 0);
+          mma_ts(t_dv, t_p, sO + so * TILE, idesc_g, t > 0, kSecond, 0);
           if (!ready(kP + 1, t & 1)) { ok = false; break; }
-          mma_ts(t_dv, t_s, sO + so * TILE, idesc_g, true, 64, 1);
+          mma_ts(t_dv, t_p, sO + so * TILE, idesc_g, true, kSecond, 1);
           if (t + 2 < n) umma_commit(bars + kEmpty + 5 + so);
           if (t + 1 < n) {
+            if (!kOwn && !read_by_now(0, t)) { ok = false; break; }
             mma_ss<NKB>(t_s, sK, sQ + ((t + 1) % 3) * TILE, idesc_s);
             umma_commit(bars + kS);
           }
           if (!ready(kDs, t & 1)) { ok = false; break; }
-          mma_ts(t_dk, t_dp, sQ + (t % 3) * TILE, idesc_g, t > 0, 64);
+          mma_ts(t_dk, t_ds, sQ + (t % 3) * TILE, idesc_g, t > 0, kSecond);
           if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
           if (t + 1 < n) {
+            if (!kOwn && !read_by_now(1, t)) { ok = false; break; }
             mma_ss<NKB>(t_dp, sV, sO + (so ^ 1) * TILE, idesc_s);
             umma_commit(bars + kDp);
           }
@@ -591,7 +605,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
             for (int c = 0; c < 16; ++c) w[c] = pack16<FMT>(p[32 * part + 2 * c], p[32 * part + 2 * c + 1]);
             __syncwarp();
-            tmem_st16(t_s + lane_addr + half * 64 + 16 * part, w);
+            tmem_st16(t_p + lane_addr + half * kSecond + 16 * part, w);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + kP + part);
@@ -627,7 +641,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 32; ++c) w[c] = pack16<FMT>(p[2 * c], p[2 * c + 1]);
         __syncwarp();
-        tmem_st32(t_dp + lane_addr + half * 64, w);
+        tmem_st32(t_ds + lane_addr + half * kSecond, w);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kDs);
@@ -728,7 +742,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
             mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0, 64);
             if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
-            if (t + 2 < n) issue_s(t + 2);
+            if (t + 2 < n) {   // over dS(t), once dQ has read it: no order of MMAs is promised
+              umma_commit(bars + kOrder);
+              if (!ready(kOrder, t & 1)) { ok = false; break; }
+              issue_s(t + 2);
+            }
           }
         } else {
           ok = ok && ready(kFull + 1, 0);
