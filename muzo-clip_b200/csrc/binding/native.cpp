@@ -69,12 +69,20 @@ void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.devic
 // Two int32 words per GPU, shared by its attention launches: [0] the first nonzero timeout code, [1]
 // a test's stall request. Created on first use; they outlive any graph, so when that use is being
 // captured they are cleared on a stream that is not.
-Tensor attention_status(int device) {
-  static std::mutex mutex;
+std::mutex status_mutex;
+Tensor& status_words(int device) {
   static std::array<Tensor, 64>* words = new std::array<Tensor, 64>;   // never destroyed: tensors must not outlive CUDA
   TORCH_CHECK(device >= 0 && device < 64, "muzo_clip_b200: GPU index ", device);
-  std::lock_guard<std::mutex> lock(mutex);
-  Tensor& t = (*words)[device];
+  return (*words)[device];
+}
+// Whether any attention launch on the GPU can have used them.
+bool attention_used(int device) {
+  std::lock_guard<std::mutex> lock(status_mutex);
+  return status_words(device).defined();
+}
+Tensor attention_status(int device) {
+  std::lock_guard<std::mutex> lock(status_mutex);
+  Tensor& t = status_words(device);
   if (!t.defined()) {
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     const auto options = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device);
@@ -434,6 +442,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_forward", &py_forward);
   m.def("attention_backward", &py_backward);
   m.def("attention_status", &attention_status);
+  m.def("attention_used", &attention_used);
   m.def("readable", [](const Tensor& t) {
     Strides s;
     const Tensor r = readable(t, s);

@@ -4,7 +4,7 @@ Drop-in for the reference package ``muzo_clip``: the same public names, signatur
 statistics, backed by the native library ``libmuzo_b200.so`` (C ABI in include/muzo_b200.h).
 """
 
-from .attention import attention_max, attention_max_backward
+from .attention import attention_max, attention_max_backward, check_attention_status
 from .grad_clip import clip_grad_norm_, clip_grads, grad_norm
 from .muzo_optimizer import MuZOClipOptimizer
 from .newton_schulz import zeropower_via_newtonschulz5
@@ -16,6 +16,7 @@ __all__ = [
     "MuZOClipOptimizer",
     "attention_max",
     "attention_max_backward",
+    "check_attention_status",
     "clip_grad_norm_",
     "clip_grads",
     "grad_norm",

@@ -21,16 +21,20 @@ _forward = _native.attention_forward
 _readable = _native.readable
 
 
+def _index(device: torch.device) -> int:
+    return device.index if device.index is not None else torch.cuda.current_device()
+
 
 def attention_status(device: torch.device) -> torch.Tensor:
     """Two device int32 words per GPU: [0] the first nonzero timeout code of an attention launch,
     [1] the stall request (0; tests set a role's code to make its first wait expire)."""
-    return _native.attention_status(device.index if device.index is not None else torch.cuda.current_device())
+    return _native.attention_status(_index(device))
 
 
 def check_attention_status(device: torch.device) -> None:
-    """Raise if an attention launch on `device` reported an expired wait (reads one word)."""
-    if device.type != "cuda":
+    """Raise if an attention launch on ``device`` reported an expired wait. Reads one word from the
+    device, and nothing where no attention has been launched."""
+    if device.type != "cuda" or not _native.attention_used(_index(device)):
         return
     t = attention_status(device)
     code = int(t[0].item())
