@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -67,8 +68,7 @@ void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.devic
 // ---------------------------------------------------------------- attention
 
 // Two int32 words per GPU, shared by its attention launches: [0] the first nonzero timeout code, [1]
-// a test's stall request. Created on first use; they outlive any graph, so when that use is being
-// captured they are cleared on a stream that is not.
+// a test's stall request. Created on first use, which may be under capture; they outlive any graph.
 std::mutex status_mutex;
 Tensor& status_words(int device) {
   static std::array<Tensor, 64>* words = new std::array<Tensor, 64>;   // never destroyed: tensors must not outlive CUDA
@@ -83,18 +83,22 @@ bool attention_used(int device) {
 Tensor attention_status(int device) {
   std::lock_guard<std::mutex> lock(status_mutex);
   Tensor& t = status_words(device);
-  if (!t.defined()) {
-    c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
-    const auto options = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device);
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-      c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
-      c10::cuda::CUDAStreamGuard side(c10::cuda::getStreamFromPool(false, static_cast<c10::DeviceIndex>(device)));
-      t = at::zeros({2}, options);
-    } else {
-      t = at::zeros({2}, options);
-      at::cuda::getCurrentCUDAStream(device).synchronize();   // cleared before another stream's launch reads them
-    }
+  if (t.defined()) return t;
+  // On a stream of their own, which no capture can be on (a stream of torch's pool may be the capturing one: the
+  // words would then lie in the graph's memory, and every replay would clear them), and cleared before any stream's
+  // launch reads them.
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
+  c10::InferenceMode normal(false);   // a check outside it clears the words
+  cudaStream_t own = nullptr;
+  C10_CUDA_CHECK(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));   // kept: the words' memory belongs to it
+  Tensor fresh;
+  {
+    c10::cuda::CUDAStreamGuard side(c10::cuda::getStreamFromExternal(own, static_cast<c10::DeviceIndex>(device)));
+    fresh = at::zeros({2}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, device));
   }
+  C10_CUDA_CHECK(cudaStreamSynchronize(own));
+  t = fresh;
   return t;
 }
 
