@@ -329,7 +329,7 @@ int muzo_max_merge(float* running, const float* fresh, const int32_t* d_valid, i
  * = dtype(dtype(max over the visible logits of q . k) * scale) and *d_valid = 0 when a visible
  * logit is non-finite, else 1. Forward only. d_status: two device int32 words, zero before the
  * first call: [0] status — a nonzero code (1 producer, 2 MMA, 3 softmax) when a bounded wait
- * expired (the outputs are then unspecified); [1] a stall request, 0 in normal use: a test sets a
+ * expired (the rows of out, and of lse below, that were computed then are NaN, *d_valid is 0); [1] a stall request, 0 in normal use: a test sets a
  * role's code there to make that role's first wait expire. */
 int muzo_attention_max(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
                        int64_t hq, int64_t hkv, int64_t seq_q, int64_t seq_k, int64_t head_dim,
@@ -364,7 +364,8 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
  * strides (batch, head, sequence) of q, k, v, out, dout, dq, dk, dv, all multiples of 8 and, for the
  * inputs, nonzero; D contiguous, bases 16-byte aligned. d_workspace: device memory of at least
  * muzo_attention_backward_workspace(...) bytes (negative: a shape this call refuses), 16-byte
- * aligned, that no other call uses until this one has finished. d_status as in muzo_attention_max. */
+ * aligned, that no other call uses until this one has finished. d_status as in muzo_attention_max: when a
+ * wait expired, the rows of dq, dk and dv that were computed then are NaN. */
 int64_t muzo_attention_backward_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t seq_q,
                                           int64_t seq_k, int64_t head_dim, int causal);
 int muzo_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* dout,

@@ -29,7 +29,7 @@
 // Visibility: key j of batch b is visible to query i when key_lo[b] <= j < key_hi[b] (padding)
 // and, when causal, j <= i + Sk - Sq. Rows without a visible key are written as zeros.
 // Every wait is bounded; on timeout the kernel records a code in the status word, raises its
-// abort flag, drains its loads and MMAs, frees TMEM and returns.
+// abort flag, drains its loads and MMAs, writes NaN to its rows, frees TMEM and returns.
 #include <atomic>
 #include <cfloat>
 #include <cstdlib>
@@ -565,6 +565,11 @@ attn_fwd_max_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       mbar_wait(drained, 0);
     }
     __syncthreads();
+    // a CTA that gave up leaves NaN in all of its rows, so that nobody takes old memory for its output
+    const int64_t row0 = static_cast<int64_t>(qb) * AMB;
+    lose_tile(static_cast<uint16_t*>(g.out) + b * g.o_sb + h * g.o_sh, g.o_ss, row0, AMB, g.sq, g.hd);
+    if (g.lse != nullptr && threadIdx.x < AMB && row0 + threadIdx.x < g.sq)
+      g.lse[(static_cast<int64_t>(b) * g.hq + h) * g.sq + row0 + threadIdx.x] = __int_as_float(0x7fffffff);
   }
   if (warp == 1) {
     tc_fence_after();

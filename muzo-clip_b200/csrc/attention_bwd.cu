@@ -296,6 +296,23 @@ __device__ __forceinline__ void give_up(const BwdArgs& g, int* abort_flag, int c
   atomicExch(abort_flag, 1);
 }
 
+// What a CTA that gave up leaves, so that nobody takes old memory or half a sum for gradients: NaN in all of its
+// rows, or in its part of the sums, which the join passes on.
+template <int D>
+__device__ __forceinline__ void lose_rows(const BwdArgs& g, bool key_cta, int kt, int bh, int b, int qt) {
+  if (!key_cta) {
+    lose_tile(g.dq + b * g.dq_sb + (bh % g.hq) * g.dq_sh, g.dq_ss, static_cast<int64_t>(qt) * AM, AM, g.sq, g.hd);
+  } else if (g.parts > 1) {
+    const int64_t part = blockIdx.x % static_cast<unsigned>(g.parts);
+    float* sums = g.partial + ((part * g.batch * g.hkv + bh) * g.nkt + kt) * AN * 2 * D;
+    for (int i = threadIdx.x; i < AN * 2 * D; i += B_THREADS) sums[i] = __int_as_float(0x7fffffff);
+  } else {
+    const int64_t key0 = static_cast<int64_t>(kt) * AN;
+    if (g.dk != nullptr) lose_tile(g.dk + b * g.dk_sb + (bh % g.hkv) * g.dk_sh, g.dk_ss, key0, AN, g.sk, g.hd);
+    if (g.dv != nullptr) lose_tile(g.dv + b * g.dv_sb + (bh % g.hkv) * g.dv_sh, g.dv_ss, key0, AN, g.sk, g.hd);
+  }
+}
+
 // Powers of two that P and dS carry on their way through 16 bits. bf16 has fp32's range and needs none.
 // In fp16 a probability below 2^-14 would lose bits, and dS, a probability times a gradient, most of them
 // (or overflow): P is taken 2^10-fold, and dS times the largest 2^k that keeps |dS| <= 2 max|dO_i| max|v_j|
@@ -883,6 +900,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       mbar_wait(drained, 0);
     }
     __syncthreads();
+    lose_rows<D>(g, key_cta, kt, bh_own, b, qt_own);
   }
   if (warp == 1) {
     tc_fence_after();

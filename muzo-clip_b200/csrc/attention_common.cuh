@@ -58,6 +58,18 @@ __device__ __forceinline__ void key_range(const int32_t* key_lo, const int32_t* 
   if (hi > sk) hi = sk;
 }
 
+// Rows [row0, row0 + rows) of a head's [S][hd] 16-bit result, as far as they exist, become NaN (0x7fff is one in
+// bf16 and in fp16). Called by all threads of a CTA.
+__device__ __forceinline__ void lose_tile(uint16_t* head, int64_t stride, int64_t row0, int rows, int64_t s, int hd) {
+  const int pieces = hd / 8;   // of 16 bytes
+  for (int i = threadIdx.x; i < rows * pieces; i += blockDim.x) {
+    const int64_t row = row0 + i / pieces;
+    if (row < s)
+      *reinterpret_cast<uint4*>(head + row * stride + 8 * (i % pieces)) =
+          make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  }
+}
+
 // 4-D tensor map over [B][H][S][D] (element strides ss, sh, sb; D contiguous), box 64 x rows. A
 // head dimension below the box's 64 or 128 columns reads zeros behind its end.
 inline int encode_attn_map(CUtensorMap* map, const void* base, int dtype, int64_t d, int64_t s, int64_t h, int64_t b,

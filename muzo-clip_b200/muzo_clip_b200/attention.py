@@ -32,16 +32,17 @@ def attention_status(device: torch.device) -> torch.Tensor:
 
 
 def check_attention_status(device: torch.device) -> None:
-    """Raise if an attention launch on ``device`` reported an expired wait. Reads one word from the
-    device, and nothing where no attention has been launched."""
+    """Raise if an attention launch on ``device`` reported an expired wait, which leaves NaN in the
+    rows of the output or of the gradients that it concerns. Reads one word from the device, and
+    nothing where no attention has been launched."""
     if device.type != "cuda" or not _native.attention_used(_index(device)):
         return
     t = attention_status(device)
     code = int(t[0].item())
     if code != 0:
         t[0].zero_()
-        raise _lib.MuzoError(f"fused attention reported status {code} (a bounded wait expired); the outputs of "
-                             "the forward that ran it are unspecified")
+        raise _lib.MuzoError(f"fused attention reported status {code} (a bounded wait expired); outputs of the forward, "
+                             "or gradients of the backward pass, that were computed then are NaN")
 
 
 def attention_max(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float | None = None,
