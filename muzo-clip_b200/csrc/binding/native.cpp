@@ -63,6 +63,14 @@ int dtype_code(const Tensor& t) {
   }
 }
 
+// Refuses what would be answered without its part: a tangent (forward-mode derivatives), torch.func's wrappers.
+void check_plain(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not supported");
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper})),
+      what, ": torch.func transforms (vmap, grad, jvp) are not supported");
+}
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // ---------------------------------------------------------------- attention
@@ -129,6 +137,7 @@ const int32_t* range_ptr(const OptTensor& t) { return t ? t->const_data_ptr<int3
 // Refuses what the kernels do not compute; returns the scaling.
 double check_attention(const Tensor& q, const Tensor& k, const Tensor& v, std::optional<double> scaling, const OptTensor& lo,
                        const OptTensor& hi) {
+  for (const Tensor* t : {&q, &k, &v}) check_plain(*t, "attention_max");
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
                     "attention_max expects 4-D query, key and value [B, H, S, D]");
   TORCH_CHECK_VALUE(q.is_cuda(), "muzo_clip_b200 attention kernels run on CUDA tensors only");
@@ -295,6 +304,7 @@ py::tuple py_forward(const Tensor& query, const Tensor& key, const Tensor& value
 py::tuple py_backward(const Tensor& grad_out, const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& out,
                       const Tensor& lse, std::optional<double> scaling, bool causal, const OptTensor& lo, const OptTensor& hi,
                       const std::array<bool, 3>& wanted) {
+  for (const Tensor* t : {&grad_out, &out, &lse}) check_plain(*t, "attention_max_backward");
   const double s = check_attention(query, key, value, scaling, lo, hi);
   const int64_t b = query.size(0), hq = query.size(1), sq = query.size(2), d = query.size(3);
   for (const Tensor* t : {&out, &grad_out})
@@ -314,6 +324,7 @@ py::tuple py_backward(const Tensor& grad_out, const Tensor& query, const Tensor&
 // The tensors' common device; none without tensors.
 std::optional<at::Device> check_grads(const std::vector<Tensor>& tensors, const char* what) {
   std::optional<at::Device> device;
+  for (const Tensor& t : tensors) check_plain(t, what);
   for (const Tensor& t : tensors) {
     TORCH_CHECK_VALUE(t.layout() == at::kStrided, what, ": sparse gradients are not supported");
     TORCH_CHECK_TYPE(dtype_code(t) >= 0, what, " supports float32, bfloat16 and float16, not ", t.scalar_type());
@@ -368,6 +379,8 @@ Tensor grad_norm(std::vector<Tensor> grads, bool inf) {
 
 // Scales grads into outs (the same list: in place) and returns the norm before.
 Tensor clip_grads(std::vector<Tensor> grads, const std::optional<std::vector<Tensor>>& outs, double max_norm, bool inf) {
+  if (outs)
+    for (const Tensor& t : *outs) check_plain(t, "clip_grads");
   const auto device = check_grads(grads, "clip_grads");
   if (outs) {
     check_grads(*outs, "clip_grads");

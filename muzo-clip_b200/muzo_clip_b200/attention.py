@@ -58,7 +58,8 @@ def attention_max(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, s
     even when it is not finite. A query that sees no key gets zeros. ``scaling`` defaults to
     D ** -0.5.
 
-    Differentiable once in query, key and value (the maxima are not): the products of the backward
+    Differentiable once, in reverse mode, in query, key and value (the maxima are not; forward-mode
+    derivatives and torch.func's transforms are refused): the products of the backward
     pass take the probabilities and their gradients in the inputs' type, as the forward does, and
     sum in fp32. A backward pass can be captured into a CUDA graph while no graph of the same leaves
     that was built on another stream is alive (torch ends such a capture with an error)."""

@@ -3,7 +3,8 @@
 ``clip_grad_norm_`` is torch's function of that name for CUDA gradients: two launches for a whole
 model, whatever the number of tensors (up to 1150 per launch), no host synchronisation, equal bits
 for equal gradients. ``clip_grads`` writes the scaled gradients elsewhere instead, in their own type
-or as fp32; ``grad_norm`` is the norm alone. Tensors of fp32, bf16 and fp16 mix freely. The native
+or as fp32; ``grad_norm`` is the norm alone. Tensors of fp32, bf16 and fp16 mix freely, on one
+device. None of the three is differentiable (as torch's clip_grad_norm_ is not). The native
 module checks the tensors (ValueError, TypeError) and makes the calls.
 """
 
