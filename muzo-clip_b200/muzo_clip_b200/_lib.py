@@ -1,7 +1,8 @@
 """ctypes binding of ``libmuzo_b200.so`` (the C ABI declared in ``include/muzo_b200.h``).
 
 The library is the only compute path of this package: if it is missing or fails to load, the
-import of this module raises and nothing falls back to PyTorch or the CPU.
+import of this module raises and nothing falls back to PyTorch or the CPU. Without the native module
+over torch tensors (``_native``) the operators that need it raise when they are called.
 """
 
 from __future__ import annotations
@@ -144,14 +145,31 @@ class MuzoError(RuntimeError):
     """A native entry point returned a non-zero status."""
 
 
+class _NativeMissing:
+    """Stands for the native module where it does not load: whatever is called of it tells why."""
+
+    def __init__(self, reason: ImportError):
+        self._reason = reason
+
+    def __getattr__(self, name):
+        def refuse(*args, **kwargs):
+            raise ImportError(
+                f"muzo_clip_b200: the native module _native failed to load ({self._reason}); build it with "
+                "`python muzo-clip_b200/build.py` against the installed torch"
+            ) from self._reason
+
+        return refuse
+
+
+# The gradient operators' calls from torch tensors. The module is built against one torch version; everything else
+# in the package goes through the C ABI above and works without it.
+native_error: ImportError | None = None
 try:
-    from . import _native as native  # the gradient operators' calls from torch tensors
+    from . import _native as native
 except ImportError as e:
-    raise ImportError(
-        f"muzo_clip_b200: the native module _native failed to load ({e}); build it with "
-        "`python muzo-clip_b200/build.py` against the installed torch"
-    ) from e
-native.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTED}, MuzoError)
+    native_error, native = e, _NativeMissing(e)
+else:
+    native.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTED}, MuzoError)
 
 
 # Kernels each compute entry point enqueues (for launch accounting by benchmarks).

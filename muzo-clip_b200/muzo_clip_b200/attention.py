@@ -35,7 +35,7 @@ def check_attention_status(device: torch.device) -> None:
     """Raise if an attention launch on ``device`` reported an expired wait, which leaves NaN in the
     rows of the output or of the gradients that it concerns. Reads one word from the device, and
     nothing where no attention has been launched."""
-    if device.type != "cuda" or not _native.attention_used(_index(device)):
+    if device.type != "cuda" or _lib.native_error is not None or not _native.attention_used(_index(device)):
         return
     t = attention_status(device)
     code = int(t[0].item())
