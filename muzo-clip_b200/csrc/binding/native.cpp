@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <cmath>
@@ -377,6 +378,93 @@ Tensor grad_norm(std::vector<Tensor> grads, bool inf) {
   return norm;
 }
 
+// Whether sum c_k z_k == target has a solution with 0 <= z_k <= m_k (c_k > 0, by descending c_k). The strides of
+// ordinary views leave one or two values to try per dimension; what takes longer counts as a solution.
+struct Term { int64_t c, m; };
+bool solvable(const std::vector<Term>& terms, size_t k, int64_t target, int64_t& budget) {
+  if (target == 0) return true;
+  if (k == terms.size() || --budget < 0) return budget < 0;
+  int64_t rest = 0;   // the largest sum of the terms behind this one
+  for (size_t i = k + 1; i < terms.size(); ++i) rest += terms[i].c * terms[i].m;
+  const int64_t c = terms[k].c;
+  const int64_t first = target > rest ? (target - rest + c - 1) / c : 0, last = std::min(terms[k].m, target / c);
+  for (int64_t z = first; z <= last; ++z)
+    if (solvable(terms, k + 1, target - c * z, budget)) return true;
+  return false;
+}
+bool solvable(std::vector<Term> terms, int64_t target) {
+  std::sort(terms.begin(), terms.end(), [](const Term& x, const Term& y) { return x.c > y.c; });
+  std::vector<Term> merged;   // equal factors are one term
+  for (const Term& t : terms) {
+    if (t.c == 0 || t.m == 0) continue;
+    if (!merged.empty() && merged.back().c == t.c) merged.back().m += t.m;
+    else merged.push_back(t);
+  }
+  int64_t budget = 1 << 16;
+  return target >= 0 && solvable(merged, 0, target, budget);
+}
+
+struct View {   // a tensor's bytes: dimensions of `m` steps of `c` bytes from `begin`, elements of `size` bytes
+  int64_t begin, end, size;
+  std::vector<Term> dims;
+  size_t tensor;
+  bool written;
+  View(const Tensor& t, size_t i, bool w)
+      : begin(reinterpret_cast<int64_t>(t.const_data_ptr())), end(0), size(t.element_size()), tensor(i), written(w) {
+    end = begin + size;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      dims.push_back({t.stride(d) * size, t.size(d) - 1});
+      end += dims.back().c * dims.back().m;
+    }
+  }
+};
+bool share_bytes(const View& a, const View& b) {   // a + x = b + y, with y counted from its end
+  std::vector<Term> terms(a.dims);
+  terms.insert(terms.end(), b.dims.begin(), b.dims.end());
+  terms.push_back({1, a.size - 1 + b.size - 1});
+  return solvable(std::move(terms), b.end - 1 - a.begin);
+}
+bool repeats_bytes(const View& v) {   // two indices, first different in dimension d, of one element
+  for (size_t d = 0; d < v.dims.size(); ++d) {
+    if (v.dims[d].m == 0) continue;
+    if (v.dims[d].c == 0) return true;
+    std::vector<Term> terms{{v.dims[d].c, v.dims[d].m - 1}};
+    int64_t target = -v.dims[d].c;
+    for (size_t e = d + 1; e < v.dims.size(); ++e) {
+      terms.push_back({v.dims[e].c, 2 * v.dims[e].m});
+      target += v.dims[e].c * v.dims[e].m;
+    }
+    if (solvable(std::move(terms), target)) return true;
+  }
+  return false;
+}
+
+// Whether anything that is written shares bytes with itself or with anything else that is written or read (a tensor
+// scaled in place is only itself), for lists in which some tensors do not fill their memory; the library
+// checks the others.
+bool any_shared(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs) {
+  std::vector<View> views;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (grads[i].numel() == 0) continue;
+    views.emplace_back(outs[i], i, true);
+    if (repeats_bytes(views.back())) return true;
+    if (!(grads[i].const_data_ptr() == outs[i].const_data_ptr() && grads[i].scalar_type() == outs[i].scalar_type() &&
+          grads[i].strides() == outs[i].strides()))
+      views.emplace_back(grads[i], i, false);
+  }
+  std::sort(views.begin(), views.end(), [](const View& x, const View& y) { return x.begin < y.begin; });
+  std::vector<const View*> open;   // those that reach beyond the present one's begin
+  for (const View& v : views) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const View* o) { return o->end <= v.begin; }), open.end());
+    for (const View* o : open)
+      if ((o->written || v.written) && share_bytes(*o, v)) return true;
+    open.push_back(&v);
+  }
+  return false;
+}
+
+constexpr char kOverlap[] = "gradient clipping: tensors that are written overlap in memory (the same one twice?)";
+
 // Scales grads into outs (the same list: in place) and returns the norm before.
 Tensor clip_grads(std::vector<Tensor> grads, const std::optional<std::vector<Tensor>>& outs, double max_norm, bool inf) {
   if (outs)
@@ -393,14 +481,16 @@ Tensor clip_grads(std::vector<Tensor> grads, const std::optional<std::vector<Ten
   std::vector<Tensor> dst = written;
   std::vector<size_t> detours;   // what does not fill its memory, or lies in another order than its output
   for (size_t i = 0; i < grads.size(); ++i) {
-    Tensor &g = grads[i], &o = dst[i];
+    const Tensor &g = grads[i], &o = dst[i];
     TORCH_CHECK_VALUE(o.device() == *device && o.sizes() == g.sizes() &&
                           (o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat),
                       "clip_grads: an output must have its gradient's shape and device, and its type or fp32");
-    if (flat(g) && (g.strides() == o.strides() || g.numel() <= 1)) continue;
-    detours.push_back(i);
-    g = g.contiguous();
-    o = at::empty(o.sizes(), o.options());
+    if (!flat(g) || (g.strides() != o.strides() && g.numel() > 1)) detours.push_back(i);
+  }
+  TORCH_CHECK_VALUE(detours.empty() || !any_shared(grads, written), kOverlap);
+  for (const size_t i : detours) {
+    grads[i] = grads[i].contiguous();
+    dst[i] = at::empty(dst[i].sizes(), dst[i].options());
   }
   const Columns from(grads), to(dst);
   const auto options = at::TensorOptions().device(*device);
@@ -410,7 +500,7 @@ Tensor clip_grads(std::vector<Tensor> grads, const std::optional<std::vector<Ten
   const int status = lib.grad_clip(from.address.data(), to.address.data(), from.numel.data(), from.dtype.data(),
                                    to.dtype.data(), static_cast<int64_t>(grads.size()), inf ? 1 : 0,
                                    static_cast<float>(max_norm), norm.data_ptr<float>(), work.data_ptr(), size, stream_of(norm));
-  TORCH_CHECK_VALUE(status != MUZO_ERR_ARG, "gradient clipping: tensors that are written overlap in memory (the same one twice?)");
+  TORCH_CHECK_VALUE(status != MUZO_ERR_ARG, kOverlap);
   check(status, "muzo_grad_clip");
   launches += 2;
   size_t next = 0;
