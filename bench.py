@@ -278,7 +278,7 @@ def _time_steps(opt, args, device, dist, local) -> dict:
 
     engine = opt._engine
     barrier()
-    launches0 = _lib.launch_count
+    launches0 = _lib.launches()
     start = torch.cuda.Event(enable_timing=True)
     end = torch.cuda.Event(enable_timing=True)
     engine.start_phase_timing()
@@ -291,7 +291,7 @@ def _time_steps(opt, args, device, dist, local) -> dict:
         barrier()
         w1 = time.perf_counter()
     phases = {k: v / args.steps for k, v in engine.stop_phase_timing().items()}
-    launches = _lib.launch_count - launches0
+    launches = _lib.launches() - launches0
     dev_ms = start.elapsed_time(end) / args.steps
     wall_ms = (w1 - w0) * 1e3 / args.steps
     if dist is not None:

@@ -99,6 +99,10 @@ int         muzo_abi_version(void);
 const char* muzo_status_string(int status);
 int         muzo_last_cuda_error(void);
 
+/* Kernels that the attention and the gradient entry points below have enqueued in this process (their number
+ * depends on the arguments; the other entry points enqueue a fixed number per call). */
+int64_t     muzo_launches(void);
+
 /* blake2b-64 of "seed|name|d0,d1|block" masked to 63 bits (prng.py:19-36). `shape` has `ndim`
  * entries. Returns the key through *key_out. Pure host code. */
 int muzo_hash64_seed(uint64_t base_seed, const char* name, const int64_t* shape, int ndim,

@@ -591,6 +591,7 @@ int launch_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap&
     configured[dev].store(true, std::memory_order_release);
   }
   kern<<<static_cast<unsigned>(g.num_items), A_THREADS, AttnLayout<D>::SMEM_BYTES, s>>>(mq, mk, mv, g);
+  count_launches(1);
   return launch_status();
 }
 
@@ -647,8 +648,10 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
     return MUZO_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int* enc = reinterpret_cast<int*>(smax);
-  if (enc != nullptr)
+  if (enc != nullptr) {
     init_attn_max_kernel<<<static_cast<unsigned>((hq + 255) / 256), 256, 0, s>>>(enc, static_cast<int>(hq), d_valid);
+    count_launches(1);
+  }
   const int64_t nqb = (seq_q + AMB - 1) / AMB;
   const int64_t items = batch * hq * nqb;
   if (items > 0) {
@@ -681,9 +684,11 @@ int muzo_attention_max_lse(const void* q, const void* k, const void* v, void* ou
       st = head_dim <= 64 ? launch_head<0, 64>(mq, mk, mv, g, s) : launch_head<0, 128>(mq, mk, mv, g, s);
     if (st != MUZO_OK) return st;
   }
-  if (enc != nullptr)
+  if (enc != nullptr) {
     finalize_attn_max_kernel<<<static_cast<unsigned>((hq + 255) / 256), 256, 0, s>>>(enc, static_cast<int>(hq), dtype,
                                                                                      scale);
+    count_launches(1);
+  }
   return launch_status();
 }
 

@@ -1076,10 +1076,12 @@ int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
   // 2048 tokens). Without a pair no statistics kernel precedes this one.
   cfg.numAttrs = g.nqt > 0 && g.nkt > 0 && g.key_items + g.query_items <= 148 ? 1 : 0;
   MUZO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, md, g));
+  count_launches(1);
   int st = launch_status();
   if (st != MUZO_OK || g.parts == 1 || g.key_items == 0) return st;
   const int64_t threads = static_cast<int64_t>(g.batch) * g.hkv * g.sk * (2 * D / 8);   // key_items <= 2^31: fewer than 2^40
   attn_bwd_join_kernel<FMT><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(g, D);
+  count_launches(1);
   return launch_status();
 }
 
@@ -1201,6 +1203,7 @@ int muzo_attention_backward(const void* q, const void* k, const void* v, const v
         Rows16{static_cast<const uint16_t*>(dout), strides[12], strides[13], strides[14]},
         Rows16{static_cast<const uint16_t*>(v), strides[6], strides[7], strides[8]}, lse, stats, largest, g.hq, seq_q, g.nqt,
         g.hd, static_cast<unsigned>(query_tiles), g.hkv, seq_k, g.nkt, d_key_lo, d_key_hi);
+    count_launches(1);
     st = launch_status();
     if (st != MUZO_OK) return st;
   }

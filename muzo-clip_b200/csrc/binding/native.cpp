@@ -16,7 +16,6 @@
 
 #include <algorithm>
 #include <array>
-#include <atomic>
 #include <cmath>
 #include <mutex>
 #include <optional>
@@ -42,7 +41,6 @@ struct Library {
   decltype(&muzo_last_cuda_error) last_cuda_error = nullptr;
 };
 Library lib;
-std::atomic<int64_t> launches{0};   // kernels enqueued by calls of this module
 
 struct Failure : std::runtime_error {
   using std::runtime_error::runtime_error;
@@ -198,7 +196,6 @@ Forward attention_forward(const Tensor& query, const Tensor& key, const Tensor& 
                               range_ptr(hi), static_cast<float*>(out_ptr(f.smax)), static_cast<int32_t*>(out_ptr(f.valid)),
                               attention_status(query.device().index()).data_ptr<int32_t>(), stream_of(query)),
         "muzo_attention_max_lse");
-  launches += record ? 3 : 1;
   return f;
 }
 
@@ -246,7 +243,6 @@ std::array<Tensor, 3> attention_backward(const Tensor& grad_out, const Tensor& q
                                static_cast<float>(scaling), range_ptr(lo), range_ptr(hi), workspace.data_ptr(), size,
                                attention_status(query.device().index()).data_ptr<int32_t>(), stream_of(query)),
         "muzo_attention_backward");
-  launches += 2;
   return grads;
 }
 
@@ -374,7 +370,6 @@ Tensor grad_norm(std::vector<Tensor> grads, bool inf) {
   check(lib.grad_norm(c.address.data(), c.numel.data(), c.dtype.data(), static_cast<int64_t>(grads.size()), inf ? 1 : 0,
                       norm.data_ptr<float>(), work.data_ptr(), size, stream_of(norm)),
         "muzo_grad_norm");
-  launches += 2;
   return norm;
 }
 
@@ -502,7 +497,6 @@ Tensor clip_grads(std::vector<Tensor> grads, const std::optional<std::vector<Ten
                                    static_cast<float>(max_norm), norm.data_ptr<float>(), work.data_ptr(), size, stream_of(norm));
   TORCH_CHECK_VALUE(status != MUZO_ERR_ARG, kOverlap);
   check(status, "muzo_grad_clip");
-  launches += 2;
   size_t next = 0;
   for (size_t i = 0; i < dst.size(); ++i) {
     if (next < detours.size() && detours[next] == i) {
@@ -544,7 +538,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     }
   });
   m.def("bind", &bind);
-  m.def("launches", [] { return launches.load(); });
   m.def("attention", &py_attention);
   m.def("attention_forward", &py_forward);
   m.def("attention_backward", &py_backward);

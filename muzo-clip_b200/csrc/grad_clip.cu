@@ -332,6 +332,7 @@ int launch_dependent(const void* kernel, unsigned grid, cudaStream_t s, void** a
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   MUZO_CUDA_CHECK(cudaLaunchKernelExC(&cfg, kernel, args));
+  count_launches(1);
   return MUZO_OK;
 }
 
@@ -372,6 +373,7 @@ int run(const Call& c, int shift, float max_norm, double* partial, float* norm, 
     void* args[] = {&t, &mine};
     MUZO_CUDA_CHECK(cudaLaunchKernel(reinterpret_cast<const void*>(grad_norm_kernel<N, INF>), dim3(grid), dim3(kThreads),
                                      args, 0, s));
+    count_launches(1);
     sums += static_cast<int>(grid);
   }
   if (c.dst == nullptr || sums == 0) {

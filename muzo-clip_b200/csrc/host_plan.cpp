@@ -17,6 +17,10 @@ static thread_local int g_last_cuda_error = 0;
 
 void set_last_cuda_error(cudaError_t err) { g_last_cuda_error = static_cast<int>(err); }
 
+static std::atomic<int64_t> g_launches{0};
+
+void count_launches(int kernels) { g_launches.fetch_add(kernels, std::memory_order_relaxed); }
+
 int device_sm_count() {
   static std::atomic<int> cached[64] = {};
   int dev = 0;
@@ -180,6 +184,8 @@ extern "C" {
 int muzo_abi_version(void) { return MUZO_ABI_VERSION; }
 
 int muzo_last_cuda_error(void) { return g_last_cuda_error; }
+
+int64_t muzo_launches(void) { return g_launches.load(std::memory_order_relaxed); }
 
 const char* muzo_status_string(int status) {
   switch (status) {

@@ -22,6 +22,10 @@ void set_last_cuda_error(cudaError_t err);
     }                                                           \
   } while (0)
 
+// Counts kernels that an entry point whose number of launches depends on its arguments has enqueued
+// (muzo_launches).
+void count_launches(int kernels);
+
 // Checks the launch that was just enqueued.
 inline int launch_status() {
   cudaError_t err = cudaGetLastError();

@@ -65,6 +65,7 @@ _SIGNATURES = {
     "muzo_abi_version": ([], _i32),
     "muzo_status_string": ([_i32], _c.c_char_p),
     "muzo_last_cuda_error": ([], _i32),
+    "muzo_launches": ([], _i64),
     "muzo_hash64_seed": ([_u64, _c.c_char_p, _vp, _i32, _i64, _vp], _i32),
     "muzo_plan_segments": ([_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _vp], _i32),
     "muzo_plan_linear": ([_vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp], _i32),
@@ -172,19 +173,23 @@ else:
     native.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTED}, MuzoError)
 
 
-# Kernels each compute entry point enqueues (for launch accounting by benchmarks).
+# Kernels each compute entry point enqueues (for launch accounting by benchmarks); those of the attention and
+# gradient entry points, whose number depends on the arguments, are counted by the library.
 KERNELS_PER_CALL = {
     "muzo_fill_noise": 1, "muzo_perturb_segments": 1, "muzo_perturb_segments_keep_noise": 1,
     "muzo_perturb_kept_noise": 1, "muzo_rebuild_segments": 1, "muzo_rebuild_segments_kept": 1,
     "muzo_ns_prepare": 1, "muzo_rebuild_segments_history": 1, "muzo_rebuild_kept_linear": 1,
     "muzo_ns_normalize": 1, "muzo_ns_gemm": 1, "muzo_update_sumsq": 1, "muzo_apply_update": 1,
     "muzo_qk_scale_rows": 1, "muzo_qk_max": 3, "muzo_qk_max_ranges": 3, "muzo_logits_head_max": 3, "muzo_max_merge": 1,
-    "muzo_ns_normalize_noalloc": 3, "muzo_attention_max": 3, "muzo_attention_max_lse": 3,
-    "muzo_attention_backward_workspace": 0, "muzo_attention_backward": 2,
-    "muzo_grad_workspace": 0, "muzo_grad_norm": 2, "muzo_grad_clip": 2, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
+    "muzo_ns_normalize_noalloc": 3, "muzo_ipc_export": 0, "muzo_ipc_import": 0, "muzo_ipc_close": 0,
     "muzo_push_blocks": 0,
 }
 launch_count = 0
+
+
+def launches() -> int:
+    """Kernels the package has enqueued so far."""
+    return launch_count + int(lib.muzo_launches())
 
 
 def launch(name: str, *args) -> None:
@@ -192,7 +197,7 @@ def launch(name: str, *args) -> None:
     global launch_count
     status = getattr(lib, name)(*args)
     check(status, name)
-    launch_count += KERNELS_PER_CALL.get(name, 1)
+    launch_count += KERNELS_PER_CALL.get(name, 0)
 
 
 def check(status: int, what: str) -> None:
