@@ -62,11 +62,14 @@ def clip_grads(grads: torch.Tensor | Iterable[torch.Tensor], max_norm: float, no
 
 
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ on the library's kernels: scales the gradients of
     ``parameters`` in place so that their norm is at most ``max_norm`` and returns the norm before.
+    The gradients are on one device and the norm is the 2-norm or the maximum; ``foreach``, torch's
+    choice between its own implementations, changes nothing here.
     A non-finite norm scales as in torch (inf: finite gradients become 0; NaN: all become NaN), or
-    raises with ``error_if_nonfinite``, which waits for the norm and leaves the gradients alone."""
+    raises with ``error_if_nonfinite``, which forms the norm first, waits for it and leaves the
+    gradients alone."""
     grads = [p.grad for p in _tensors(parameters) if p.grad is not None]
     if error_if_nonfinite:
         _max_norm(max_norm)
