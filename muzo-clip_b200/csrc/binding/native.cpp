@@ -64,7 +64,8 @@ int dtype_code(const Tensor& t) {
 
 // Refuses what would be answered without its part: a tangent (forward-mode derivatives), torch.func's wrappers.
 void check_plain(const Tensor& t, const char* what) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not supported");
+  if (t.unsafeGetTensorImpl()->autograd_meta() != nullptr)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not supported");
   TORCH_CHECK_NOT_IMPLEMENTED(
       !t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper})),
       what, ": torch.func transforms (vmap, grad, jvp) are not supported");
