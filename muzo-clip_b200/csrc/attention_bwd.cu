@@ -471,6 +471,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     constexpr int kSecond = kOwn ? 32 : 64;   // columns from the first 64 K rows to the others
     const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = t_dv + D;
     const uint32_t t_p = kOwn ? tmem + 384 : t_s, t_ds = kOwn ? tmem + 448 : t_dp;
+    // The first rows of a head's first tile may see no key (left padding under causality, more queries than keys).
+    // Their P and dS are 0, but 0 times a non-finite dO or Q would still reach dV and dK: warp 2 clears those rows
+    // before the products.
+    const int64_t blind = g.causal ? lo - g.shift - static_cast<int64_t>(first) * AM : 0;
+    const int blind_rows = n > 0 && blind > 0 ? static_cast<int>(blind) : 0;   // fewer than a tile's: `first` sees a key
 
     if (warp == 0) {
       if (lane == 0 && n > 0) {
@@ -509,9 +514,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           mma_ss<NKB>(t_dp, sV, sO, idesc_s);
           umma_commit(bars + kDp);
         }
-        for (int t = 0; t < n && ok; ++t) {
+        for (int t = 0, pos = begin % count; t < n && ok; ++t, pos = pos + 1 < count ? pos + 1 : 0) {
           const int so = t & 1;
-          // P(t) written, S(t) read, the next Q and dO loaded (warp 2 arrives for them): dV, then the next S
+          // P(t) written, S(t) read, the next Q and dO loaded and rows cleared (warp 2 arrives for them): dV, then
+          // the next S
+          if (blind_rows > 0 && pos == 0 && !ready(kP + 1, t & 1)) { ok = false; break; }
           if (!ready(kP, t & 1)) { ok = false; break; }
           mma_ts(t_dv, t_p, sO + so * TILE, idesc_g, t > 0, kSecond, 0);
           if (!ready(kP + 1, t & 1)) { ok = false; break; }
@@ -537,26 +544,39 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       __syncwarp();
     } else if (warp == 2) {
       // Waits for the loads in the issuer's place: its polls queue behind the MMAs it has issued (150 to
-      // 270 cycles each, with the tensor cores idle), so it is left with two per tile.
-      if (lane == 0 && n > 0) {
-        bool ok = true;
-        for (int t = 0; t < n && ok; ++t) {
-          if (t > 0) ok = wait_one<false>(bars + kP + 1, (t - 1) & 1, abort_flag);
+      // 270 cycles each, with the tensor cores idle), so it is left with two per tile. And clears the rows of Q and dO
+      // that see no key.
+      bool ok = true;
+      for (int t = 0, pos = n > 0 ? begin % count : 0; t < n && ok; ++t, pos = pos + 1 < count ? pos + 1 : 0) {
+        if (lane == 0 && t > 0) ok = wait_one<false>(bars + kP + 1, (t - 1) & 1, abort_flag);
+        if (blind_rows > 0 && pos == 0) {
+          if (lane == 0) ok = ok && wait_one<false>(bars + kDp, t & 1, abort_flag);   // S(t) and dP(t) have read them
+          if (__shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0) {
+            uint8_t *q_rows = sQ + (t % 3) * TILE, *o_rows = sO + (t & 1) * TILE;   // contiguous in each block of 64 columns
+            for (int i = lane; i < 8 * blind_rows; i += 32)
+#pragma unroll
+              for (int kb = 0; kb < NKB; ++kb) {
+                *reinterpret_cast<uint4*>(q_rows + kb * SUB_BYTES + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(o_rows + kb * SUB_BYTES + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
           if (ok && t + 1 < n)
             ok = wait_one<false>(bars + kFull + 2 + (t + 1) % 3, ((t + 1) / 3) & 1, abort_flag) &&
                  wait_one<false>(bars + kFull + 5 + ((t + 1) & 1), ((t + 1) >> 1) & 1, abort_flag);
           if (ok) mbar_arrive(bars + kP + 1);
         }
-        if (!ok) give_up(g, abort_flag, kErrTimeoutMma);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
+      if (!ok && lane == 0) give_up(g, abort_flag, kErrTimeoutMma);
       __syncwarp();
     } else if (warp >= 4) {
       const Powers two = n > 0 ? powers_of<FMT>(g) : Powers();
       const int64_t key = static_cast<int64_t>(kt) * AN + r;
       const bool key_seen = key >= lo && key < hi;
-      const int64_t blind = g.causal ? lo - g.shift : 0;   // rows in front of the first that sees a key
-      const int blind_rows = blind > 0 ? static_cast<int>(blind % AM) : 0;
-      const int blind_tile = blind_rows > 0 ? static_cast<int>(blind / AM) : -1;
       bool ok = true;
       if (stall == kErrTimeoutEpilogue) {
         bool waited = true;
@@ -580,20 +600,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           break;
         }
         tc_fence_after();
-        // The first rows of a head's first tile may see no key (left padding under causality, more queries than
-        // keys). Their P and dS are 0, but 0 times a non-finite dO or Q would still reach dV and dK, so those rows
-        // are cleared: dO's once dP(t) has read them, Q's (S(t) has read them) now.
-        if (qt == blind_tile) {
-          if (half == 0 && !warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
-          if (r < blind_rows) {
-            uint8_t* row = (half == 0 ? sO + so * TILE : sQ + sq * TILE) + r * 128;
-#pragma unroll
-            for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(row + kb * SUB_BYTES + 16 * e) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-        }
         const float4* nl = reinterpret_cast<const float4*>(neg_lse + so * 128 + half * 64);
         const float4* dl = reinterpret_cast<const float4*>(neg_delta + sq * 128 + half * 64);
         float p[64];
