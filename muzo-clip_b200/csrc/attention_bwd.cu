@@ -899,11 +899,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (*reinterpret_cast<volatile int*>(abort_flag)) {   // every role has ended: the same answer in all threads
-    // the MMAs that an aborted CTA issued end before its TMEM is released (bounded)
+    // the MMAs that an aborted CTA issued end before its TMEM is released (bounded), and the arrivals of commits that
+    // nobody waits for any more, which have no stated order, get 50 us
     if ((warp == 1 || warp == 2) && elect_one()) {
       uint64_t* drained = bars + kDrain + (warp == 1 ? 0 : 1);
       umma_commit(drained);
       mbar_wait(drained, 0);
+      mbar_wait(bars + kStall, 0, kSettleCycles);
     }
     __syncthreads();
     lose_rows<D>(g, key_cta, kt, bh_own, b, qt_own);

@@ -15,6 +15,7 @@ constexpr unsigned long long kWaitLimitCycles = 4ull * 1000 * 1000 * 1000;  // ~
 // A stall request (test use: a status word a kernel reads at start) makes the named role wait on
 // a barrier nothing arrives at, for kStallLimitCycles, and then take the timeout path.
 constexpr unsigned long long kStallLimitCycles = kWaitLimitCycles / 8;
+constexpr unsigned long long kSettleCycles = 100 * 1000;   // 50 us: what an aborted CTA leaves to asynchronous arrivals
 
 enum : int { kErrNone = 0, kErrTimeoutProducer = 1, kErrTimeoutMma = 2, kErrTimeoutEpilogue = 3 };
 
