@@ -21,11 +21,11 @@
 //
 // What bounds it, at head dimension 128: a key CTA's pair of tiles is a chain, S -> P (1100 cycles, of
 // which the special-function unit's 1024) -> dV -> next S (1024 of tensor work), about 2700 cycles with
-// the hand-overs for 2048 of tensor work; dS, dK and the next dP run beside it. A query CTA's pair takes
-// about 2400 for 1536: P and dS in turn in the same warps. TMEM (512 columns: S, dP, dV, dK, or
-// two S, dP, dQ) leaves no second buffer to break the chains. A Llama-3-70B-shaped layer (4096 tokens, 64 and
-// 8 heads, causal): 0.80 ms, 860 TFLOP/s of the five products, 1200 of the seven; one of 2048 tokens with 32
-// and 8 heads: 0.123 ms. Over seconds the GPU's 1000 W set the pace (1.55 GHz).
+// the hand-overs for 2048 of tensor work, and the commits that tell of dV and dK on top (3 to 11 % of this kernel's
+// time); dS, dK and the next dP run beside it. A query CTA's pair takes about 2500 for 1536: P and dS in turn in
+// the same warps. TMEM (512 columns: S, dP, dV, dK, or two S, dP, dQ) leaves no second buffer to break the chains.
+// A Llama-3-70B-shaped layer (4096 tokens, 64 and 8 heads, causal): 0.87 ms, 790 TFLOP/s of the five products, 1110
+// of the seven; one of 2048 tokens with 32 and 8 heads: 0.132 ms. Over seconds the GPU's 1000 W set the pace.
 #include <atomic>
 #include <cfloat>
 
@@ -37,8 +37,8 @@ namespace {
 using namespace tc;
 using namespace attn;
 
-constexpr int B_THREADS = 384;   // warp 0 TMA, warps 1 and 2 MMA, warps 4..11 probabilities: two groups of
-                                 // four, one warp of each per TMEM lane quarter
+constexpr int B_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warp 2 waits for a key CTA's loads, warps 4..11
+                                 // probabilities: two groups of four, one warp of each per TMEM lane quarter
 constexpr uint32_t B_TMEM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -119,32 +119,11 @@ __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, const i
   }
   return true;
 }
-// A look at a barrier ahead of time, without a branch: lane 0 polls, the answer is used later by
-// `looked_or_wait`. A poll queues behind the exponentials of both warps of a scheduler (300 cycles and
-// more), which pass meanwhile.
-__device__ __forceinline__ uint32_t look(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.eq.u32 q, %3, 0;\n\t"
-      "mov.u32 %0, 0;\n\t"
-      "@q mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "@q selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(threadIdx.x & 31)
-      : "memory");
-  return done;
-}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const int* abort_flag) {
   bool ready = true;
   if ((threadIdx.x & 31) == 0) ready = wait_one(bar, parity, abort_flag);
   __syncwarp();
   return __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
-}
-
-__device__ __forceinline__ bool looked_or_wait(uint32_t looked, uint64_t* bar, uint32_t parity, const int* abort_flag) {
-  if (__shfl_sync(0xffffffffu, looked, 0) != 0) return true;
-  return warp_wait(bar, parity, abort_flag);
 }
 
 // Query tiles [first, first + count) that see a key of key tile kt in batch row b.
@@ -231,10 +210,10 @@ enum : int {
                     // next tile's loads are here. Query CTA, the first: dP read
   kDs = 19,         // dS written, and in a key CTA dP read (query CTA: two, by buffer: its readers run apart)
   kDone = 21,
-  kDrain = 22,      // two: one per issuer
-  kStall = 24,
-  kOrder = 25,      // two: a product has read its A operand from TMEM, and the next S or dP may take the columns
-  kBars = 27
+  kDrain = 22,
+  kStall = 23,
+  kOrder = 24,      // two: a product has read its A operand from TMEM, and the next S or dP may take the columns
+  kBars = 26
 };
 
 // Loads issued by the producer thread: which full barriers are armed, and with which parity.
@@ -360,13 +339,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const bool key_cta = static_cast<int64_t>(blockIdx.x) < g.key_items;
 
   if (threadIdx.x == 0) {
-    // One thread initialises every barrier, and no load is issued before the CTA's barrier below. (Initialised by a
-    // lane each, and used by the first loads behind a __syncwarp, they began 2 to 4 us earlier, but nothing ordered
-    // the other lanes' initialisations before the loads' arrivals: a launch in some ten thousand faulted.)
+    // One thread initialises every barrier, and no load is issued before the CTA's barrier below. (Loads issued 2 to 4
+    // us earlier, behind barriers that a lane each had initialised, were part of a form whose launches faulted now and
+    // then; what made them fault was not shown.)
     // arrivals: the eight probability warps on kP and kDs, the warp that waits for a key CTA's loads on its second
-    // kP, a query CTA's two issuers on kDone
-    for (int i = 0; i < kBars; ++i)
-      mbar_init(bars + i, i == kP + 1 ? 9 : (i >= kP && i < kDone ? 8 : (i == kDone && !key_cta ? 2 : 1)));
+    // kP
+    for (int i = 0; i < kBars; ++i) mbar_init(bars + i, i == kP + 1 ? 9 : (i >= kP && i < kDone ? 8 : 1));
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -740,44 +718,46 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         armed.wait_all(bars);
       }
       __syncwarp();
-    } else if (warp == 1 || warp == 2) {
-      // Two issuers: warp 1 dQ(t), S(t+2) into the buffer of dS(t); warp 2 dP(t+1) once dP(t) is read.
+    } else if (warp == 1) {
+      // One issuer, as in a key CTA. (A second warp for the dP products and polls ahead of time in the probability
+      // warps made a long backward pass 4 % faster. Only grids with query CTAs are known to have faulted, rarely and
+      // from a cause that was not shown, and these were what query CTAs had beside a key CTA's parts.)
       if (n > 0 && elect_one()) {
         auto ready = [&](int bar, uint32_t parity) -> bool {
           if (!wait_one(bars + bar, parity, abort_flag)) return false;
           tc_fence_after();
           return true;
         };
+        auto issue_s = [&](int t) {
+          mma_ss<NKB>(t_s + 128 * (t & 1), sQ, sK + (t % 3) * TILE, idesc_s);
+          umma_commit(bars + kS + (t & 1));
+        };
+        auto issue_dp = [&](int t) {
+          mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
+          umma_commit(bars + kDp);
+          if (t + 2 < n) umma_commit(bars + kEmpty + 5 + (t & 1));
+        };
         bool ok = stall != kErrTimeoutMma || mbar_wait(bars + kStall, 0, kStallLimitCycles);
-        if (warp == 1) {
-          auto issue_s = [&](int t) {
-            mma_ss<NKB>(t_s + 128 * (t & 1), sQ, sK + (t % 3) * TILE, idesc_s);
-            umma_commit(bars + kS + (t & 1));
-          };
-          ok = ok && ready(kFull, 0) && ready(kFull + 2, 0);
-          if (ok) issue_s(0);
-          if (ok && n > 1) {
-            ok = ready(kFull + 3, 0);
-            if (ok) issue_s(1);
+        ok = ok && ready(kFull, 0) && ready(kFull + 2, 0);
+        if (ok) issue_s(0);
+        ok = ok && ready(kFull + 1, 0) && ready(kFull + 5, 0);
+        if (ok) issue_dp(0);
+        if (ok && n > 1) {
+          ok = ready(kFull + 3, 0);
+          if (ok) issue_s(1);
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          if (t + 1 < n) {   // dP(t) read: the next one
+            if (!ready(kFull + 5 + ((t + 1) & 1), ((t + 1) >> 1) & 1) || !ready(kP, t & 1)) { ok = false; break; }
+            issue_dp(t + 1);
           }
-          for (int t = 0; t < n && ok; ++t) {
-            if (t + 2 < n && !ready(kFull + 2 + (t + 2) % 3, ((t + 2) / 3) & 1)) { ok = false; break; }
-            if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
-            mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0, 64);
-            if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
-            if (t + 2 < n) {   // over dS(t), once dQ has read it: no order of MMAs is promised
-              umma_commit(bars + kOrder);
-              if (!ready(kOrder, t & 1)) { ok = false; break; }
-              issue_s(t + 2);
-            }
-          }
-        } else {
-          ok = ok && ready(kFull + 1, 0);
-          for (int t = 0; t < n && ok; ++t) {
-            if (!ready(kFull + 5 + (t & 1), (t >> 1) & 1) || (t > 0 && !ready(kP, (t - 1) & 1))) { ok = false; break; }
-            mma_ss<NKB>(t_dp, sO, sV + (t & 1) * TILE, idesc_s);
-            umma_commit(bars + kDp);
-            if (t + 2 < n) umma_commit(bars + kEmpty + 5 + (t & 1));
+          if (!ready(kDs + (t & 1), (t >> 1) & 1)) { ok = false; break; }
+          mma_ts(t_dq, t_s + 128 * (t & 1), sK + (t % 3) * TILE, idesc_g, t > 0, 64);
+          if (t + 3 < n) umma_commit(bars + kEmpty + 2 + t % 3);
+          if (t + 2 < n) {   // S(t+2) over dS(t), once dQ has read it: no order of MMAs is promised
+            umma_commit(bars + kOrder);
+            if (!ready(kOrder, t & 1) || !ready(kFull + 2 + (t + 2) % 3, ((t + 2) / 3) & 1)) { ok = false; break; }
+            issue_s(t + 2);
           }
         }
         if (ok) umma_commit(bars + kDone);
@@ -800,7 +780,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (lane == 0) waited = mbar_wait(bars + kStall, 0, kStallLimitCycles);
         ok = __shfl_sync(0xffffffffu, waited ? 1 : 0, 0) != 0;
       }
-      uint32_t s_here = 0;   // a look at the next S
       for (int t = 0; t < n && ok; ++t) {
         const int64_t key0 = static_cast<int64_t>(first + t) * AN;
         const int64_t a0 = lo - key0 - 64 * half, a1 = end - key0 - 64 * half;
@@ -808,17 +787,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int c_hi = a1 < 0 ? 0 : (a1 > 64 ? 64 : static_cast<int>(a1));
         const bool all_seen = __all_sync(0xffffffffu, c_lo == 0 && c_hi == 64);
         const uint32_t my_s = t_s + 128 * (t & 1) + lane_addr + half * 64;
-        if (!looked_or_wait(s_here, bars + kS + (t & 1), (t >> 1) & 1, abort_flag)) { ok = false; break; }
+        if (!warp_wait(bars + kS + (t & 1), (t >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         float p[64];
-        uint32_t dp_here;
         {
           uint32_t v[64];
           __syncwarp();
           tmem_ld64(my_s, v);
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
-            if (c == 32) dp_here = look(bars + kDp, t & 1);
             p[c] = __uint_as_float(v[c]);
             p[c + 1] = __uint_as_float(v[c + 1]);
             fma_pair(p[c], p[c + 1], g.scale_log2, nl, nl);
@@ -826,7 +803,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             p[c + 1] = fast_exp2(p[c + 1]);
           }
         }
-        if (!looked_or_wait(dp_here, bars + kDp, t & 1, abort_flag)) { ok = false; break; }
+        if (!warp_wait(bars + kDp, t & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         {
           uint32_t v[64];
@@ -835,7 +812,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + kP);   // dP(t) read: the next one may be formed
-          s_here = look(bars + kS + ((t + 1) & 1), ((t + 1) >> 1) & 1);
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
             float x0 = __uint_as_float(v[c]), x1 = __uint_as_float(v[c + 1]);
@@ -901,10 +877,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   if (*reinterpret_cast<volatile int*>(abort_flag)) {   // every role has ended: the same answer in all threads
     // the MMAs that an aborted CTA issued end before its TMEM is released (bounded), and the arrivals of commits that
     // nobody waits for any more, which have no stated order, get 50 us
-    if ((warp == 1 || warp == 2) && elect_one()) {
-      uint64_t* drained = bars + kDrain + (warp == 1 ? 0 : 1);
-      umma_commit(drained);
-      mbar_wait(drained, 0);
+    if (warp == 1 && elect_one()) {
+      umma_commit(bars + kDrain);
+      mbar_wait(bars + kDrain, 0);
       mbar_wait(bars + kStall, 0, kSettleCycles);
     }
     __syncthreads();
@@ -1079,8 +1054,8 @@ int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
-  // Early only where all CTAs fit at once: 17.4 -> 11.7 us for 27 of them. With 640, launched early, the short
-  // query CTAs ran before the long key CTAs instead of beside them: 152 against 124 us (32 and 8 heads,
+  // Early only where all CTAs fit at once: 15.5 -> 11.9 us for 27 of them when it came. With 640, launched early, the
+  // short query CTAs ran before the long key CTAs instead of beside them: 152 against 124 us (32 and 8 heads,
   // 2048 tokens). Without a pair no statistics kernel precedes this one.
   cfg.numAttrs = g.nqt > 0 && g.nkt > 0 && g.key_items + g.query_items <= 148 ? 1 : 0;
   MUZO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, md, g));
@@ -1097,7 +1072,7 @@ int launch_bwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
 // fewest with which the longest key CTA does not outlast the average SM by more than 15 % (a division
 // costs the sums' way through memory and a launch). In units of one pair of a key CTA, a pair of a query
 // CTA takes 0.85 and a CTA's start and end 2.5 (2800, 2400 and 7000 cycles); causal CTAs start longest
-// first, and the short query CTAs fill what is left. Measured, us for 1 / 2 / 3 / 4 / 8 parts: 32 query
+// first, and the short query CTAs fill what is left. Measured (before the commits of kOrder), us for 1 / 2 / 3 / 4 / 8 parts: 32 query
 // and 8 key heads, 2048 tokens 125 / 146 / 157 / 167 / 198; 8 and 1 heads, 2048 tokens 226 / 122 / 88 /
 // 71 / 45; 8 and 1 heads, 16384 tokens 1783 / 1476 / 1583 / 1569 / 1491.
 int64_t key_parts(int64_t batch, int64_t hkv, int64_t group, int64_t nqt, int64_t nkt, bool causal, bool queries) {
