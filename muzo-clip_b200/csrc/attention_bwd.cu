@@ -925,7 +925,8 @@ struct Rows16 {   // a [B][H][S][D] operand of 16-bit elements
 // Per query row: -lse in log2 units (with the power of two that P carries; -inf for a row that sees no
 // key, so that its probabilities are 0) and -delta = -dO . O, in tiles of 128 rows padded with such rows: one
 // block per tile, 16 lanes per row (8 elements each), four rows per lane with their loads in flight
-// together. For fp16 also the largest |dO_i|^2 of the rows that see a key and, in the blocks behind the query
+// together. O is what the caller has, 16 bits: its rounding leaves an error of dO . (half a step of O) in delta, which
+// dP - delta does not outgrow where P is close to one-hot. For fp16 also the largest |dO_i|^2 of the rows that see a key and, in the blocks behind the query
 // tiles', the largest |v_j|^2 of the keys inside their range.
 template <int FMT>
 __global__ void __launch_bounds__(kStatThreads, 2)

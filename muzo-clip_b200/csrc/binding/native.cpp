@@ -1,6 +1,6 @@
 // Python module muzo_clip_b200._native: the gradient operators' calls from torch tensors to the C
 // ABI, with their checks of arguments, their outputs and workspaces (torch's allocator, the current
-// stream of the tensors' device) and their autograd node. A call's host side takes 5 to 15 us this
+// stream of the tensors' device) and their autograd node. A call's host side takes 9 to 16 us this
 // way; the same steps in Python over ctypes took 30 to 60 us, and 200 us with the backward pass
 // behind the interpreter lock: more than the kernels of a small model.
 //

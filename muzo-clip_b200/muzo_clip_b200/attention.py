@@ -55,14 +55,20 @@ def attention_max(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, s
 
     ``causal``: query i sees the keys j <= i + Sk - Sq. ``key_lo`` / ``key_hi`` (int32 per batch)
     bound the visible keys to [key_lo, key_hi); what lies outside is not read into any result, not
-    even when it is not finite. A query that sees no key gets zeros. ``scaling`` defaults to
+    even when it is not finite (a key that only causality hides is multiplied by a probability of 0, so
+    a NaN in it does reach queries of its tile). A query that sees no key gets zeros, and gives nothing
+    to any gradient. ``scaling`` defaults to
     D ** -0.5.
 
     Differentiable once, in reverse mode, in query, key and value (the maxima are not; forward-mode
-    derivatives and torch.func's transforms are refused): the products of the backward
-    pass take the probabilities and their gradients in the inputs' type, as the forward does, and
-    sum in fp32. A backward pass can be captured into a CUDA graph while no graph of the same leaves
-    that was built on another stream is alive (torch ends such a capture with an error)."""
+    derivatives and torch.func's transforms are refused): the products of the backward pass take the
+    probabilities and their gradients in the inputs' type, as the forward does, and sum in fp32;
+    dO . O is taken from the output as it is returned, rounded to the inputs' type. That rounding is
+    what a row of query's gradient loses most by where one key has nearly all of its probability:
+    dP - dO . O cancels, and the row, small itself, may be off by its own size.
+
+    A backward pass can be captured into a CUDA graph while no graph of the same leaves that was built
+    on another stream is alive (torch ends such a capture with an error)."""
     return _native.attention(query, key, value, scaling, causal, key_lo, key_hi, record)
 
 
